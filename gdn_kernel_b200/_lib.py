@@ -21,6 +21,9 @@ GDN_B200_OK = 0
 GDN_B200_ERR_INVALID_ARGUMENT = 1
 GDN_B200_ERR_CUDA = 2
 
+BF16, FP16, FP32 = 0, 1, 2                       # element types of the mixer operators
+ACT_NONE, ACT_SILU, ACT_SIGMOID = 0, 1, 2
+
 STATUS_TMA_TIMEOUT = 1
 STATUS_MMA_TIMEOUT = 2
 STATUS_BAD_SEQLENS = 4
@@ -29,6 +32,8 @@ STATUS_SELFTEST_WAIT = 16
 
 # Every symbol the header declares, with its ctypes signature.
 _P = ctypes.c_void_p
+_L = ctypes.c_int64
+_I = ctypes.c_int32
 _SIGNATURES = {
     "gdn_b200_decode": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_double, _P, _P,
                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
@@ -63,6 +68,20 @@ _SIGNATURES = {
                                               ctypes.c_int32, ctypes.c_int32, _P, ctypes.c_uint64,
                                               _P]),
     "gdn_b200_state_affine": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int64, _P]),
+    "gdn_b200_short_conv": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _I, _P, _I, _P, _L, _P, _L, _L,
+                                 _L, _I, _I, _I, _P]),
+    "gdn_b200_short_conv_step": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _P, _L, _P, _L, _L, _I, _I,
+                                      _I, _P]),
+    "gdn_b200_ssm_prefill_workspace_size": (ctypes.c_uint64, [_L, _L, _I, _I, _I]),
+    "gdn_b200_ssm_prefill": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _P, _P, _P, _I, _P, _I,
+                                  _P, _P, _P, _L, _L, _L, _I, _I, _I, _I, _P, ctypes.c_uint64,
+                                  _P]),
+    "gdn_b200_ssm_step": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _P, _P,
+                               _L, _L, _I, _I, _I, _I, _P]),
+    "gdn_b200_gated_norm": (_I, [_P, _L, _P, _L, _P, _I, _P, _L, _L, _I, _I, ctypes.c_double, _I,
+                                 _I, _I, _P]),
+    "gdn_b200_add_norm": (_I, [_P, _L, _P, _L, _P, _P, _P, ctypes.c_double, _P, _L, _P, _L, _L, _I,
+                               ctypes.c_double, ctypes.c_double, _I, _I, _P]),
     "gdn_b200_current_device": (ctypes.c_int32, []),
     "gdn_b200_device_status": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint32),
                                               ctypes.c_int32]),

@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -22,7 +23,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
+NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
               "--expt-relaxed-constexpr"]
 
 LIB = os.path.join(PKG, "libgdn_b200.so")
@@ -61,15 +62,27 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
     """Compile every shared library of the package; returns their paths."""
     core_deps = _sources("gdn_b200.cu", "gdn_ptx.cuh", "decode_kernel.cuh", "prefill_kernel.cuh",
                          "prefill_split.cuh", "state_affine_kernel.cuh")
-    core_deps.append(os.path.join(INCLUDE, "gdn_b200.h"))
-    if force or _stale(LIB, core_deps):
-        cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, f"-I{INCLUDE}", "-o", LIB,
-               os.path.join(CSRC, "gdn_b200.cu")]
-        if ptxas_verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        out = _run(cmd, verbose)
-        if ptxas_verbose:
-            print(out)
+    shared = [os.path.join(CSRC, "host_common.h"), os.path.join(INCLUDE, "gdn_b200.h")]
+    mixer_deps = _sources("mixer.cu", "gdn_ptx.cuh", "mixer_common.cuh", "short_conv.cuh",
+                          "ssm_recurrent.cuh", "block_norm.cuh")
+    units = [("gdn_b200.cu", core_deps + shared), ("mixer.cu", mixer_deps + shared)]
+    objects, stale = [], []
+    for src, deps in units:
+        obj = os.path.join(PKG, os.path.splitext(src)[0] + ".o")
+        objects.append(obj)
+        if force or _stale(obj, deps):
+            cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, "-c", f"-I{INCLUDE}", "-o", obj,
+                   os.path.join(CSRC, src)]
+            if ptxas_verbose:
+                cmd.insert(1, "-Xptxas=-v")
+            stale.append(cmd)
+    # the units compile side by side
+    with ThreadPoolExecutor() as pool:
+        for out in pool.map(lambda cmd: _run(cmd, verbose), stale):
+            if ptxas_verbose:
+                print(out)
+    if force or _stale(LIB, objects):
+        _run([_nvcc(), *ARCH, "-shared", "-o", LIB, *objects], verbose)
     built = [LIB]
     try:
         import tvm_ffi  # noqa: F401

@@ -13,6 +13,7 @@
 #include <string>
 
 #include "gdn_b200.h"
+#include "host_common.h"
 #include "decode_kernel.cuh"
 #include "prefill_split.cuh"
 #include "state_affine_kernel.cuh"
@@ -145,6 +146,37 @@ float resolve_scale(double scale) {
 }
 
 }  // namespace
+
+// The same for the library's other translation units (host_common.h): nothing
+// may leave a C entry point as an exception.
+int lib_fail(int code, const char* msg) noexcept {
+  try {
+    t_last_error = msg;
+  } catch (...) {
+  }
+  return code;
+}
+
+int lib_cuda_fail(cudaError_t e, const char* what) noexcept {
+  try {
+    return cuda_fail(e, what);
+  } catch (...) {
+    return GDN_B200_ERR_CUDA;
+  }
+}
+
+void lib_clear_error() noexcept { t_last_error.clear(); }
+
+int lib_device(unsigned int** status, int* sm_count) noexcept {
+  try {
+    if (int rc = device_setup(status)) return rc;
+    *sm_count = device_sm_count();
+    return GDN_B200_OK;
+  } catch (...) {
+    return lib_fail(GDN_B200_ERR_CUDA, "device setup failed");
+  }
+}
+
 }  // namespace gdn
 
 using namespace gdn;

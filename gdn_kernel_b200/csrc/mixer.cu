@@ -1,0 +1,457 @@
+// C-ABI entry points of the operators around a recurrent block (declared in
+// include/gdn_b200.h): short causal convolution, selective state space scan,
+// gated norm, residual add and norm.  Host-side validation and launches.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "gdn_b200.h"
+#include "host_common.h"
+#include "block_norm.cuh"
+#include "short_conv.cuh"
+#include "ssm_recurrent.cuh"
+
+namespace gdn {
+namespace {
+
+constexpr long long kMaxGrid = 0x7fffffffLL;
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
+int invalid(const char* msg) { return lib_fail(GDN_B200_ERR_INVALID_ARGUMENT, msg); }
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? GDN_B200_OK : lib_cuda_fail(e, what);
+}
+
+int element_size(int32_t dtype) {
+  return dtype == GDN_B200_BF16 || dtype == GDN_B200_FP16 ? 2 : dtype == GDN_B200_FP32 ? 4 : 0;
+}
+
+// Rows of `stride` elements that 16-byte accesses can walk.
+bool wide_rows(const void* p, long long stride, int size) {
+  return aligned(p, 16) && stride * size % 16 == 0;
+}
+
+// ------------------------------------------------------------ short convolution
+template <typename T, int V, int W>
+void launch_conv(ConvParams& p, long long blocks_per_chan, bool step, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>(blocks_per_chan * p.chan_blocks);
+  if (step) gdn_short_conv_step_kernel<T, V, W><<<grid, kConvThreads, 0, st>>>(p);
+  else gdn_short_conv_kernel<T, V, W><<<grid, kConvThreads, 0, st>>>(p);
+}
+
+template <typename T, int V>
+void launch_conv_width(ConvParams& p, int width, long long n, bool step, cudaStream_t st) {
+  if (width == 2) launch_conv<T, V, 2>(p, n, step, st);
+  else if (width == 3) launch_conv<T, V, 3>(p, n, step, st);
+  else launch_conv<T, V, 4>(p, n, step, st);
+}
+
+template <typename T>
+int launch_conv_type(ConvParams& p, int width, long long n, bool step, cudaStream_t st) {
+  const int size = static_cast<int>(sizeof(T));
+  // 16-byte vectors where every row starts on one, else one channel per thread
+  const bool wide = p.channels % kLanes<T> == 0 && wide_rows(p.x, p.x_stride, size) &&
+                    wide_rows(p.out, p.out_stride, size) && aligned(p.weight, 16) &&
+                    aligned(p.bias, 16) && aligned(p.state, 16) && aligned(p.new_state, 16);
+  const int v = wide ? kLanes<T> : 1;
+  p.chan_blocks = (p.channels / v + kConvThreads - 1) / kConvThreads;
+  if (n > kMaxGrid / p.chan_blocks) return invalid("tokens * channels exceeds the grid limit");
+  if (wide) launch_conv_width<T, kLanes<T>>(p, width, n, step, st);
+  else launch_conv_width<T, 1>(p, width, n, step, st);
+  return launched("short convolution launch");
+}
+
+int conv_call(ConvParams& p, int width, int32_t dtype, long long n, bool step, void* stream) {
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == GDN_B200_BF16) return launch_conv_type<__nv_bfloat16>(p, width, n, step, st);
+  if (dtype == GDN_B200_FP16) return launch_conv_type<__half>(p, width, n, step, st);
+  return launch_conv_type<float>(p, width, n, step, st);
+}
+
+int check_conv(int64_t rows, int64_t pool, int32_t channels, int32_t width, int32_t dtype,
+               int32_t activation) {
+  if (!element_size(dtype)) return invalid("dtype must be GDN_B200_BF16, _FP16 or _FP32");
+  if (activation != GDN_B200_ACT_NONE && activation != GDN_B200_ACT_SILU)
+    return invalid("activation must be GDN_B200_ACT_NONE or _SILU");
+  if (width < 2 || width > 4) return invalid("width must be 2, 3 or 4");
+  if (channels < 1 || channels > (1 << 24)) return invalid("channels must be in [1, 2^24]");
+  if (rows < 0 || pool < 0) return invalid("extents must be >= 0");
+  return GDN_B200_OK;
+}
+
+// ------------------------------------------------------------ norms
+template <typename T, int kTeam, int kVecs>
+void launch_gated(const NormParams& p, long long groups, cudaStream_t st) {
+  constexpr int per_block = kTeam > 32 ? 1 : kNormThreads / kTeam;
+  gdn_gated_norm_kernel<T, kLanes<T>, kTeam, kVecs>
+      <<<static_cast<unsigned>((groups + per_block - 1) / per_block),
+         kTeam > 32 ? kTeam : kNormThreads, 0, st>>>(p);
+}
+
+template <typename T>
+int gated_call(const NormParams& p, cudaStream_t st) {
+  const long long groups = p.rows * (p.width / p.group);
+  if (groups > kMaxGrid) return invalid("rows * groups exceeds the grid limit");
+  const int size = static_cast<int>(sizeof(T));
+  const bool wide = p.group % kLanes<T> == 0 && wide_rows(p.x, p.x_stride, size) &&
+                    (!p.gate || wide_rows(p.gate, p.gate_stride, size)) &&
+                    wide_rows(p.out, p.out_stride, size) && aligned(p.weight, 16);
+  const int nv = p.group / kLanes<T>;
+  if (!wide || nv > 4096) gdn_gated_norm_any_kernel<T><<<static_cast<unsigned>(groups), 256, 0, st>>>(p);
+  else if (nv <= 8) launch_gated<T, 8, 1>(p, groups, st);
+  else if (nv <= 16) launch_gated<T, 16, 1>(p, groups, st);
+  else if (nv <= 32) launch_gated<T, 32, 1>(p, groups, st);
+  else if (nv <= 64) launch_gated<T, 32, 2>(p, groups, st);
+  else if (nv <= 128) launch_gated<T, 32, 4>(p, groups, st);
+  else if (nv <= 512) launch_gated<T, 256, 2>(p, groups, st);
+  else if (nv <= 1024) launch_gated<T, 512, 2>(p, groups, st);
+  else launch_gated<T, 1024, 4>(p, groups, st);
+  return launched("gated norm launch");
+}
+
+template <typename T, typename R, int kTeam, int kVecs>
+void launch_add(const NormParams& p, cudaStream_t st) {
+  constexpr int per_block = kTeam > 32 ? 1 : kNormThreads / kTeam;
+  gdn_add_norm_kernel<T, R, kLanes<T>, kTeam, kVecs>
+      <<<static_cast<unsigned>((p.rows + per_block - 1) / per_block),
+         kTeam > 32 ? kTeam : kNormThreads, 0, st>>>(p);
+}
+
+template <typename T, typename R>
+int add_call(const NormParams& p, cudaStream_t st) {
+  if (p.rows > kMaxGrid) return invalid("rows exceeds the grid limit");
+  const int size = static_cast<int>(sizeof(T)), rsize = static_cast<int>(sizeof(R));
+  const bool wide = p.width % kLanes<T> == 0 && wide_rows(p.x, p.x_stride, size) &&
+                    wide_rows(p.out, p.out_stride, size) &&
+                    wide_rows(p.residual, p.residual_stride, rsize) &&
+                    wide_rows(p.new_residual, p.new_residual_stride, rsize) &&
+                    aligned(p.weight, 16) && aligned(p.block_weight, 16);
+  const int nv = p.width / kLanes<T>;
+  if (!wide || nv > 4096) gdn_add_norm_any_kernel<T, R><<<static_cast<unsigned>(p.rows), 256, 0, st>>>(p);
+  else if (nv <= 32) launch_add<T, R, 32, 1>(p, st);
+  else if (nv <= 64) launch_add<T, R, 32, 2>(p, st);
+  else if (nv <= 128) launch_add<T, R, 64, 2>(p, st);
+  else if (nv <= 256) launch_add<T, R, 128, 2>(p, st);
+  else if (nv <= 512) launch_add<T, R, 256, 2>(p, st);
+  else if (nv <= 1024) launch_add<T, R, 512, 2>(p, st);
+  else launch_add<T, R, 1024, 4>(p, st);
+  return launched("add norm launch");
+}
+
+// ------------------------------------------------------------ selective scan
+int check_ssm(int64_t rows, int64_t pool, int32_t heads, int32_t groups, int32_t head_dim,
+              int32_t state_dim) {
+  if (head_dim != 64 && head_dim != 128) return invalid("head_dim must be 64 or 128");
+  if (state_dim != 64 && state_dim != 128) return invalid("state_dim must be 64 or 128");
+  if (heads < 1 || groups < 1 || heads % groups != 0)
+    return invalid("num_heads must be a positive multiple of num_groups");
+  if (heads > 65535) return invalid("num_heads exceeds 65535");
+  if (rows < 0 || pool < 0) return invalid("extents must be >= 0");
+  return GDN_B200_OK;
+}
+
+int check_ssm_rows(const SsmParams& p) {
+  if (!p.x || !p.dt || !p.B || !p.C || !p.A_log || !p.out) return invalid("null pointer argument");
+  if (!wide_rows(p.x, p.x_stride, 2) || !wide_rows(p.B, p.b_stride, 2) ||
+      !wide_rows(p.C, p.c_stride, 2) || !aligned(p.out, 16))
+    return invalid("x, B, C and output need 16-byte aligned rows");
+  return GDN_B200_OK;
+}
+
+template <bool kPrompt>
+int ssm_recurrent_call(const SsmParams& p, int32_t state_dim, int64_t entries, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.heads * (p.head_dim / kSsmBlockRows)),
+                  static_cast<unsigned>(entries));
+  if (state_dim == 64) gdn_ssm_recurrent_kernel<64, kPrompt><<<grid, kSsmThreads, 0, st>>>(p);
+  else gdn_ssm_recurrent_kernel<128, kPrompt><<<grid, kSsmThreads, 0, st>>>(p);
+  return launched("selective scan launch");
+}
+
+}  // namespace
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_b200_short_conv(const void* x, int64_t x_stride, const void* weight,
+                                   const void* bias, const void* state, const void* cu_seqlens,
+                                   int32_t cu_seqlens_is_int64, const void* state_indices,
+                                   int32_t indices_are_int64, const uint8_t* has_state,
+                                   int32_t activation, void* output, int64_t output_stride,
+                                   void* new_state, int64_t num_seqs, int64_t total_tokens,
+                                   int64_t pool_size, int32_t channels, int32_t width,
+                                   int32_t dtype, void* stream) {
+  lib_clear_error();
+  if (int rc = check_conv(total_tokens, pool_size, channels, width, dtype, activation)) return rc;
+  if (num_seqs < 0 || num_seqs > kMaxGrid) return invalid("num_seqs must be in [0, 2^31)");
+  if (num_seqs == 0) return GDN_B200_OK;
+  if (!weight || !cu_seqlens || !new_state || (total_tokens > 0 && (!x || !output)))
+    return invalid("null pointer argument");
+  if (total_tokens > 1 && (x_stride < channels || output_stride < channels))
+    return invalid("rows must not overlap");
+  if (!state_indices && pool_size < num_seqs)
+    return invalid("the states hold fewer rows than there are sequences");
+  if (!aligned(cu_seqlens, cu_seqlens_is_int64 ? 8 : 4) ||
+      !aligned(state_indices, indices_are_int64 ? 8 : 4))
+    return invalid("cu_seqlens or state_indices is misaligned");
+  ConvParams p{};
+  int sms = 0;
+  if (int rc = lib_device(&p.status, &sms)) return rc;
+  p.x = x;
+  p.weight = weight;
+  p.bias = bias;
+  p.state = state;
+  p.new_state = new_state;
+  p.out = output;
+  p.cu = cu_seqlens;
+  p.slots = state_indices;
+  p.has_state = has_state;
+  p.x_stride = x_stride;
+  p.out_stride = output_stride;
+  p.pool = pool_size;
+  p.tokens = total_tokens;
+  p.cu_is64 = cu_seqlens_is_int64 ? 1 : 0;
+  p.slots_is64 = indices_are_int64 ? 1 : 0;
+  p.seqs = static_cast<int>(num_seqs);
+  p.channels = channels;
+  p.silu = activation == GDN_B200_ACT_SILU;
+  const long long tiles = std::max<long long>(1, (total_tokens + kConvTile - 1) / kConvTile);
+  return conv_call(p, width, dtype, tiles, false, stream);
+}
+
+extern "C" int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const void* weight,
+                                        const void* bias, const void* state_pool,
+                                        const void* state_indices, int32_t indices_are_int64,
+                                        int32_t activation, void* output, int64_t output_stride,
+                                        void* new_state_pool, int64_t batch, int64_t pool_size,
+                                        int32_t channels, int32_t width, int32_t dtype,
+                                        void* stream) {
+  lib_clear_error();
+  if (int rc = check_conv(batch, pool_size, channels, width, dtype, activation)) return rc;
+  if (batch == 0) return GDN_B200_OK;
+  if (!x || !weight || !state_pool || !new_state_pool || !output)
+    return invalid("null pointer argument");
+  if (batch > 1 && (x_stride < channels || output_stride < channels))
+    return invalid("rows must not overlap");
+  if (!state_indices && pool_size < batch)
+    return invalid("the states hold fewer rows than there are batch entries");
+  if (!aligned(state_indices, indices_are_int64 ? 8 : 4))
+    return invalid("state_indices is misaligned");
+  ConvParams p{};
+  int sms = 0;
+  if (int rc = lib_device(&p.status, &sms)) return rc;
+  p.x = x;
+  p.weight = weight;
+  p.bias = bias;
+  p.state = state_pool;
+  p.new_state = new_state_pool;
+  p.out = output;
+  p.slots = state_indices;
+  p.x_stride = x_stride;
+  p.out_stride = output_stride;
+  p.pool = pool_size;
+  p.tokens = batch;
+  p.slots_is64 = indices_are_int64 ? 1 : 0;
+  p.channels = channels;
+  p.silu = activation == GDN_B200_ACT_SILU;
+  return conv_call(p, width, dtype, batch, true, stream);
+}
+
+extern "C" uint64_t gdn_b200_ssm_prefill_workspace_size(int64_t, int64_t, int32_t, int32_t,
+                                                        int32_t) {
+  return 0;
+}
+
+extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void* dt,
+                                    int64_t dt_stride, const float* A_log, const void* B,
+                                    int64_t b_stride, const void* C, int64_t c_stride,
+                                    const float* D, const float* dt_bias, const float* state,
+                                    const void* cu_seqlens, int32_t cu_seqlens_is_int64,
+                                    const void* state_indices, int32_t indices_are_int64,
+                                    const uint8_t* has_state, void* output, float* new_state,
+                                    int64_t num_seqs, int64_t total_tokens, int64_t pool_size,
+                                    int32_t num_heads, int32_t num_groups, int32_t head_dim,
+                                    int32_t state_dim, void* workspace, uint64_t workspace_bytes,
+                                    void* stream) {
+  lib_clear_error();
+  (void)workspace;
+  (void)workspace_bytes;
+  if (int rc = check_ssm(total_tokens, pool_size, num_heads, num_groups, head_dim, state_dim))
+    return rc;
+  if (num_seqs < 0 || num_seqs > 65535) return invalid("num_seqs must be in [0, 65535]");
+  if (num_seqs == 0) return GDN_B200_OK;
+  if (!cu_seqlens || !new_state) return invalid("null pointer argument");
+  if (!state_indices && pool_size < num_seqs)
+    return invalid("the states hold fewer rows than there are sequences");
+  if (!aligned(cu_seqlens, cu_seqlens_is_int64 ? 8 : 4) ||
+      !aligned(state_indices, indices_are_int64 ? 8 : 4))
+    return invalid("cu_seqlens or state_indices is misaligned");
+  if (!aligned(state, 16) || !aligned(new_state, 16))
+    return invalid("state and new_state need 16-byte alignment");
+  SsmParams p{};
+  int sms = 0;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.dt = static_cast<const __nv_bfloat16*>(dt);
+  p.B = static_cast<const __nv_bfloat16*>(B);
+  p.C = static_cast<const __nv_bfloat16*>(C);
+  p.A_log = A_log;
+  p.D = D;
+  p.dt_bias = dt_bias;
+  p.state = state;
+  p.new_state = new_state;
+  p.out = static_cast<__nv_bfloat16*>(output);
+  p.cu = cu_seqlens;
+  p.slots = state_indices;
+  p.has_state = has_state;
+  p.x_stride = x_stride;
+  p.dt_stride = dt_stride;
+  p.b_stride = b_stride;
+  p.c_stride = c_stride;
+  p.pool = pool_size;
+  p.tokens = total_tokens;
+  p.cu_is64 = cu_seqlens_is_int64 ? 1 : 0;
+  p.slots_is64 = indices_are_int64 ? 1 : 0;
+  p.seqs = static_cast<int>(num_seqs);
+  p.heads = num_heads;
+  p.groups = num_groups;
+  p.head_dim = head_dim;
+  if (!A_log) return invalid("null pointer argument");
+  if (total_tokens > 0)
+    if (int rc = check_ssm_rows(p)) return rc;
+  if (int rc = lib_device(&p.status, &sms)) return rc;
+  return ssm_recurrent_call<true>(p, state_dim, num_seqs, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int gdn_b200_ssm_step(const void* x, int64_t x_stride, const void* dt,
+                                 int64_t dt_stride, const float* A_log, const void* B,
+                                 int64_t b_stride, const void* C, int64_t c_stride, const float* D,
+                                 const float* dt_bias, const float* state_pool,
+                                 const void* read_indices, const void* write_indices,
+                                 int32_t indices_are_int64, void* output, float* new_state_pool,
+                                 int64_t batch, int64_t pool_size, int32_t num_heads,
+                                 int32_t num_groups, int32_t head_dim, int32_t state_dim,
+                                 void* stream) {
+  lib_clear_error();
+  if (int rc = check_ssm(batch, pool_size, num_heads, num_groups, head_dim, state_dim)) return rc;
+  if (batch > 65535) return invalid("batch exceeds 65535");
+  if (batch == 0) return GDN_B200_OK;
+  if (!state_pool || !new_state_pool) return invalid("null pointer argument");
+  if (!read_indices && pool_size < batch)
+    return invalid("the states hold fewer rows than there are batch entries");
+  if (!read_indices && write_indices) return invalid("write_indices need read_indices");
+  if (!aligned(read_indices, indices_are_int64 ? 8 : 4) ||
+      !aligned(write_indices, indices_are_int64 ? 8 : 4))
+    return invalid("state indices are misaligned");
+  if (!aligned(state_pool, 16) || !aligned(new_state_pool, 16))
+    return invalid("the state pools need 16-byte alignment");
+  SsmParams p{};
+  int sms = 0;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.dt = static_cast<const __nv_bfloat16*>(dt);
+  p.B = static_cast<const __nv_bfloat16*>(B);
+  p.C = static_cast<const __nv_bfloat16*>(C);
+  p.A_log = A_log;
+  p.D = D;
+  p.dt_bias = dt_bias;
+  p.state = state_pool;
+  p.new_state = new_state_pool;
+  p.out = static_cast<__nv_bfloat16*>(output);
+  p.slots = read_indices;
+  p.write_slots = write_indices;
+  p.x_stride = x_stride;
+  p.dt_stride = dt_stride;
+  p.b_stride = b_stride;
+  p.c_stride = c_stride;
+  p.pool = pool_size;
+  p.tokens = batch;
+  p.slots_is64 = indices_are_int64 ? 1 : 0;
+  p.heads = num_heads;
+  p.groups = num_groups;
+  p.head_dim = head_dim;
+  if (int rc = check_ssm_rows(p)) return rc;
+  if (int rc = lib_device(&p.status, &sms)) return rc;
+  return ssm_recurrent_call<false>(p, state_dim, batch, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int gdn_b200_gated_norm(const void* x, int64_t x_stride, const void* gate,
+                                   int64_t gate_stride, const void* weight,
+                                   int32_t weight_is_shared, void* output, int64_t output_stride,
+                                   int64_t rows, int32_t width, int32_t group_size, double eps,
+                                   int32_t activation, int32_t norm_first, int32_t dtype,
+                                   void* stream) {
+  lib_clear_error();
+  if (!element_size(dtype)) return invalid("dtype must be GDN_B200_BF16, _FP16 or _FP32");
+  if (rows < 0 || width < 1 || group_size < 1 || width % group_size != 0)
+    return invalid("width must be a positive multiple of group_size");
+  if (activation != GDN_B200_ACT_SILU && activation != GDN_B200_ACT_SIGMOID)
+    return invalid("activation must be GDN_B200_ACT_SILU or _SIGMOID");
+  if (!(eps >= 0.0)) return invalid("eps must be >= 0");
+  if (rows == 0) return GDN_B200_OK;
+  if (!x || !output) return invalid("null pointer argument");
+  if (rows > 1 && (x_stride < width || output_stride < width || (gate && gate_stride < width)))
+    return invalid("rows must not overlap");
+  NormParams p{};
+  p.x = x;
+  p.gate = gate;
+  p.weight = weight;
+  p.weight_shared = weight_is_shared ? 1 : 0;
+  p.out = output;
+  p.rows = rows;
+  p.x_stride = x_stride;
+  p.gate_stride = gate_stride;
+  p.out_stride = output_stride;
+  p.width = width;
+  p.group = group_size;
+  p.silu = activation == GDN_B200_ACT_SILU;
+  p.norm_first = norm_first ? 1 : 0;
+  p.eps = static_cast<float>(eps);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == GDN_B200_BF16) return gated_call<__nv_bfloat16>(p, st);
+  if (dtype == GDN_B200_FP16) return gated_call<__half>(p, st);
+  return gated_call<float>(p, st);
+}
+
+extern "C" int gdn_b200_add_norm(const void* x, int64_t x_stride, const void* residual,
+                                 int64_t residual_stride, const void* weight,
+                                 const void* block_weight, const float* channel_scale,
+                                 double scale, void* output, int64_t output_stride,
+                                 void* new_residual, int64_t new_residual_stride, int64_t rows,
+                                 int32_t width, double eps, double weight_offset, int32_t dtype,
+                                 int32_t residual_is_fp32, void* stream) {
+  lib_clear_error();
+  if (!element_size(dtype)) return invalid("dtype must be GDN_B200_BF16, _FP16 or _FP32");
+  if (rows < 0 || width < 1) return invalid("rows must be >= 0 and width >= 1");
+  if (!(eps >= 0.0)) return invalid("eps must be >= 0");
+  if (rows == 0) return GDN_B200_OK;
+  if (!x || !residual || !weight || !output || !new_residual)
+    return invalid("null pointer argument");
+  if (rows > 1 && (x_stride < width || residual_stride < width || output_stride < width ||
+                   new_residual_stride < width))
+    return invalid("rows must not overlap");
+  NormParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.block_weight = block_weight;
+  p.channel_scale = channel_scale;
+  p.out = output;
+  p.new_residual = new_residual;
+  p.rows = rows;
+  p.x_stride = x_stride;
+  p.residual_stride = residual_stride;
+  p.out_stride = output_stride;
+  p.new_residual_stride = new_residual_stride;
+  p.width = width;
+  p.eps = static_cast<float>(eps);
+  p.scale = static_cast<float>(scale);
+  p.weight_offset = static_cast<float>(weight_offset);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == GDN_B200_FP32) return add_call<float, float>(p, st);
+  if (dtype == GDN_B200_BF16)
+    return residual_is_fp32 ? add_call<__nv_bfloat16, float>(p, st)
+                            : add_call<__nv_bfloat16, __nv_bfloat16>(p, st);
+  return residual_is_fp32 ? add_call<__half, float>(p, st) : add_call<__half, __half>(p, st);
+}

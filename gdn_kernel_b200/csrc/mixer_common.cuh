@@ -1,0 +1,110 @@
+// What the mixer kernels share: 16-byte vectors of the three element types, and
+// the lookup of the packed sequence that a token tile belongs to.
+#pragma once
+
+#include <cstdint>
+#include <type_traits>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace gdn {
+
+// Status bits, as in the GDN kernels.
+constexpr unsigned int kMixerBadSeqlens = 4u;
+constexpr unsigned int kMixerBadIndex = 8u;
+
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+
+// N consecutive elements as they lie in memory: one 16-byte access, or a single
+// element where sizes or addresses allow no wider one.
+template <typename T, int N>
+struct Pack {
+  static constexpr bool kWide = N * sizeof(T) == 16;
+  using Raw = typename std::conditional<kWide, uint4, T>::type;
+  static_assert(kWide || N == 1, "one 16-byte vector or one element");
+  Raw raw;
+
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
+  // Read once: no line kept in L1.
+  __device__ __forceinline__ void load_stream(const T* p) {
+    if constexpr (kWide) raw = __ldcs(reinterpret_cast<const uint4*>(p));
+    else raw = *p;
+  }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void zero() {
+    if constexpr (kWide) raw = make_uint4(0u, 0u, 0u, 0u);
+    else raw = from_float<T>(0.0f);
+  }
+  __device__ __forceinline__ void unpack(float (&f)[N]) const {
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_float(e[i]);
+  }
+  __device__ __forceinline__ void pack(const float (&f)[N]) {
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = from_float<T>(f[i]);
+  }
+};
+
+// Elements of a 16-byte vector.
+template <typename T> constexpr int kLanes = 16 / static_cast<int>(sizeof(T));
+
+// v sigmoid(v) and sigmoid(v); exp(-v) = inf gives 0 as it should.
+__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float silu_f(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+
+__device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
+  return is64 ? reinterpret_cast<const long long*>(p)[i]
+              : static_cast<long long>(reinterpret_cast<const int*>(p)[i]);
+}
+
+// The slot of entry i: the entry itself without indices; -1 for a padding entry
+// (negative) and for one past the pool, which also raises the status bit.
+__device__ __forceinline__ long long slot_of(const void* idx, int is64, long long i,
+                                             long long pool, unsigned int* status, bool report) {
+  if (idx == nullptr) return i;
+  const long long s = index_at(idx, is64, i);
+  if (s >= pool) {
+    if (report) atomicOr(status, kMixerBadIndex);
+    return -1;
+  }
+  return s < 0 ? -1 : s;
+}
+
+// One block reports offsets that do not rise within [0, tokens].
+__device__ __forceinline__ void check_offsets(const void* cu, int is64, int n, long long tokens,
+                                              unsigned int* status) {
+  bool bad = false;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const long long s = index_at(cu, is64, i), e = index_at(cu, is64, i + 1);
+    bad |= s < 0 || e < s || e > tokens;
+  }
+  if (bad) atomicOr(status, kMixerBadSeqlens);
+}
+
+// How many of the first n entries of the non-decreasing cu are below t: a
+// 32-way search by one whole warp, one load of cu per lane and level.
+__device__ __forceinline__ int count_below(const void* cu, int is64, int n, long long t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;   // entries before lo are below t, entries from hi on are not
+  while (lo < hi) {
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const bool below = at < hi && index_at(cu, is64, at) < t;
+    const int k = __popc(__ballot_sync(0xffffffffu, below));   // probes below t: a prefix
+    if (k == 0) return lo;
+    lo = lo + (k - 1) * step + 1;
+    hi = min(hi, lo - 1 + step);
+  }
+  return lo;
+}
+
+}  // namespace gdn

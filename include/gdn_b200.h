@@ -44,6 +44,14 @@ extern "C" {
 #define GDN_B200_STATUS_BAD_INDEX 8u     /* a state-pool index was >= pool_size */
 #define GDN_B200_STATUS_SELFTEST_WAIT 16u /* gdn_b200_selftest_wait_timeout's wait ran out */
 
+/* Element types and activations of the mixer operators (short convolution, norms). */
+#define GDN_B200_BF16 0
+#define GDN_B200_FP16 1
+#define GDN_B200_FP32 2
+#define GDN_B200_ACT_NONE 0
+#define GDN_B200_ACT_SILU 1
+#define GDN_B200_ACT_SIGMOID 2
+
 /*
  * One T=1 decode step for `batch` sequences.
  * Replaces the reference's TVM-FFI `kernel` of solution/cuda/kernel.cu:101-150
@@ -236,6 +244,121 @@ int gdn_b200_prefill_static(const void* q, const void* k, const void* v, const f
                             double scale, void* output, float* new_state,
                             int64_t num_seqs, int64_t total_tokens, int32_t num_qk_heads,
                             int32_t num_v_heads, int32_t head_dim, void* stream);
+
+/*
+ * ------------------------------------------------------------ mixer operators
+ * What stands around a recurrent block in a serving model.  No counterpart in
+ * the reference.  Row strides count elements and let an operand be a column
+ * slice of a wider activation; the elements of a row are contiguous.  A state
+ * pool is contiguous.  With `state_indices` ([N] or [batch], int32 or int64)
+ * sequence i's state is that slot of the pool, else slot i.  A negative index
+ * means no slot: prompts then start from zero and store no state, a batch entry
+ * of a step is padding (zero output, no state read or written).  An index >=
+ * pool_size counts as negative and raises GDN_B200_STATUS_BAD_INDEX.  Slots
+ * written by one call must be distinct, and none may be read by another entry.
+ * New states may be written in place.  Offsets that do not rise within
+ * [0, total_tokens] raise GDN_B200_STATUS_BAD_SEQLENS; such sequences are
+ * skipped.  Tokens outside [cu_seqlens[0], cu_seqlens[N]) are not written.
+ */
+
+/*
+ * Short causal convolution per channel over packed prompts, width W in 2..4:
+ *   y_t = act(bias + sum_k weight[:, k] * u_{t-(W-1)+k}),
+ * u being the sequence's carried rows, then its tokens.
+ *   x, output    [T, channels] of `dtype`;  weight [channels, W], bias [channels] or NULL
+ *   state        [pool_size, W-1, channels] (oldest row first), NULL = zero
+ *   new_state    the same shape: the last W-1 rows of u; may be `state`
+ *   has_state    [N] bytes or NULL: sequences whose byte is 0 start from zero
+ * output must not overlap x.  activation: GDN_B200_ACT_NONE or _SILU.
+ */
+int gdn_b200_short_conv(const void* x, int64_t x_stride, const void* weight, const void* bias,
+                        const void* state, const void* cu_seqlens, int32_t cu_seqlens_is_int64,
+                        const void* state_indices, int32_t indices_are_int64,
+                        const uint8_t* has_state, int32_t activation, void* output,
+                        int64_t output_stride, void* new_state, int64_t num_seqs,
+                        int64_t total_tokens, int64_t pool_size, int32_t channels, int32_t width,
+                        int32_t dtype, void* stream);
+
+/*
+ * The same for one new token per sequence: x, output [batch, channels] (output
+ * may be x), state_pool and new_state_pool [pool_size, W-1, channels] (may be
+ * the same).
+ */
+int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const void* weight, const void* bias,
+                             const void* state_pool, const void* state_indices,
+                             int32_t indices_are_int64, int32_t activation, void* output,
+                             int64_t output_stride, void* new_state_pool, int64_t batch,
+                             int64_t pool_size, int32_t channels, int32_t width, int32_t dtype,
+                             void* stream);
+
+/*
+ * Selective state space scan over packed prompts.  Per head, state h [P, N]:
+ *   step = softplus(dt + dt_bias);  h <- exp(-exp(A_log) step) h + (step x) B^T;
+ *   y = h C + D x.
+ *   x, output    [T, H, P] bf16 (output contiguous);  dt [T, H] bf16
+ *   B, C         [T, G, N] bf16; head h reads group h / (H / G)
+ *   A_log [H] fp32;  D, dt_bias [H] fp32 or NULL (zero)
+ *   state, new_state [pool_size, H, P, N] fp32; state NULL = zero; may be the same
+ *   head_dim P in {64, 128}, state_dim N in {64, 128}, H % G == 0
+ * x, B and C need 16-byte aligned rows.  An empty sequence keeps its state.
+ * The workspace (gdn_b200_ssm_prefill_workspace_size() bytes, 256-byte aligned)
+ * lets long sequences run in pieces side by side; NULL is allowed.  Calls that
+ * may overlap need workspaces of their own.
+ */
+uint64_t gdn_b200_ssm_prefill_workspace_size(int64_t num_seqs, int64_t total_tokens,
+                                             int32_t num_heads, int32_t head_dim,
+                                             int32_t state_dim);
+int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,
+                         const float* A_log, const void* B, int64_t b_stride, const void* C,
+                         int64_t c_stride, const float* D, const float* dt_bias,
+                         const float* state, const void* cu_seqlens, int32_t cu_seqlens_is_int64,
+                         const void* state_indices, int32_t indices_are_int64,
+                         const uint8_t* has_state, void* output, float* new_state,
+                         int64_t num_seqs, int64_t total_tokens, int64_t pool_size,
+                         int32_t num_heads, int32_t num_groups, int32_t head_dim,
+                         int32_t state_dim, void* workspace, uint64_t workspace_bytes,
+                         void* stream);
+
+/*
+ * The same for one new token per sequence: x [batch, H, P], dt [batch, H],
+ * B, C [batch, G, N].  write_indices NULL: the read slots.
+ */
+int gdn_b200_ssm_step(const void* x, int64_t x_stride, const void* dt, int64_t dt_stride,
+                      const float* A_log, const void* B, int64_t b_stride, const void* C,
+                      int64_t c_stride, const float* D, const float* dt_bias,
+                      const float* state_pool, const void* read_indices,
+                      const void* write_indices, int32_t indices_are_int64, void* output,
+                      float* new_state_pool, int64_t batch, int64_t pool_size, int32_t num_heads,
+                      int32_t num_groups, int32_t head_dim, int32_t state_dim, void* stream);
+
+/*
+ * Norm after a mixer with its gate, by groups of a row, rms(v) = v / sqrt(mean(v^2) + eps):
+ *   norm_first:  y = rms(x) weight act(gate);   else  y = rms(x act(gate)) weight
+ *   x, gate, output [rows, width] of `dtype`; gate NULL = no gate; output may be x or gate
+ *   weight  [group_size] (weight_is_shared) or [width] of `dtype`, NULL = ones
+ * activation: GDN_B200_ACT_SILU or _SIGMOID.
+ */
+int gdn_b200_gated_norm(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                        const void* weight, int32_t weight_is_shared, void* output,
+                        int64_t output_stride, int64_t rows, int32_t width, int32_t group_size,
+                        double eps, int32_t activation, int32_t norm_first, int32_t dtype,
+                        void* stream);
+
+/*
+ * Residual add and the next block's norm:
+ *   r' = residual + s u,  u = x, or rms(x) block_weight where that is given;
+ *   output = rms(r') (weight + weight_offset)
+ * s: channel_scale [width] fp32, or `scale` where that is NULL.  x, weight,
+ * block_weight and output are of `dtype`; residual and new_residual of `dtype`
+ * or fp32; the norm reads r' before it is rounded.  new_residual may be
+ * residual, output may be x.
+ */
+int gdn_b200_add_norm(const void* x, int64_t x_stride, const void* residual,
+                      int64_t residual_stride, const void* weight, const void* block_weight,
+                      const float* channel_scale, double scale, void* output,
+                      int64_t output_stride, void* new_residual, int64_t new_residual_stride,
+                      int64_t rows, int32_t width, double eps, double weight_offset,
+                      int32_t dtype, int32_t residual_is_fp32, void* stream);
 
 /*
  * Reads (and with clear != 0 resets) the status word that the kernels of

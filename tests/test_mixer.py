@@ -1,0 +1,159 @@
+"""The mixer operators' refusals, at the C entry and in Python (no GPU needed),
+and their oracle against torch's own forms."""
+
+import ctypes
+
+import pytest
+import torch
+
+from gdn_kernel_b200 import _lib, mixer as M
+from oracle import mixer_oracle as O
+
+Z = ctypes.c_void_p(0)
+BAD = _lib.GDN_B200_ERR_INVALID_ARGUMENT
+
+
+def _conv(lib, n=1, t=4, pool=1, channels=64, width=4, dtype=_lib.BF16, act=1, xs=64):
+    return lib.gdn_b200_short_conv(Z, xs, Z, Z, Z, Z, 0, Z, 0, Z, act, Z, xs, Z, n, t, pool,
+                                   channels, width, dtype, Z)
+
+
+def _conv_step(lib, b=2, pool=2, channels=64, width=4, dtype=_lib.BF16, act=1):
+    return lib.gdn_b200_short_conv_step(Z, 64, Z, Z, Z, Z, 0, act, Z, 64, Z, b, pool, channels,
+                                        width, dtype, Z)
+
+
+def _scan(lib, n=1, t=4, pool=1, H=4, G=1, P=64, N=128):
+    return lib.gdn_b200_ssm_prefill(Z, 1, Z, 1, Z, Z, 1, Z, 1, Z, Z, Z, Z, 0, Z, 0, Z, Z, Z, n, t,
+                                    pool, H, G, P, N, Z, 0, Z)
+
+
+def _scan_step(lib, b=2, pool=2, H=4, G=1, P=64, N=128):
+    return lib.gdn_b200_ssm_step(Z, 1, Z, 1, Z, Z, 1, Z, 1, Z, Z, Z, Z, Z, 0, Z, Z, b, pool, H, G,
+                                 P, N, Z)
+
+
+def _gated(lib, rows=2, width=128, group=64, eps=1e-6, act=1, dtype=0):
+    return lib.gdn_b200_gated_norm(Z, width, Z, width, Z, 1, Z, width, rows, width, group, eps, act,
+                                   1, dtype, Z)
+
+
+def _add(lib, rows=2, width=128, eps=1e-6, dtype=0):
+    return lib.gdn_b200_add_norm(Z, width, Z, width, Z, Z, Z, 1.0, Z, width, Z, width, rows, width,
+                                 eps, 0.0, dtype, 0, Z)
+
+
+@pytest.mark.parametrize("fn,kw,word", [
+    (_conv, dict(width=5), b"width"), (_conv, dict(width=1), b"width"),
+    (_conv, dict(channels=0), b"channels"), (_conv, dict(dtype=3), b"dtype"),
+    (_conv, dict(act=2), b"activation"), (_conv, dict(t=-1), b"extents"),
+    (_conv, dict(n=-1), b"num_seqs"), (_conv, {}, b"null"),
+    (_conv_step, dict(width=7), b"width"), (_conv_step, dict(b=-1), b"extents"),
+    (_conv_step, {}, b"null"),
+    (_scan, dict(P=96), b"head_dim"), (_scan, dict(N=32), b"state_dim"),
+    (_scan, dict(H=5, G=2), b"multiple"), (_scan, dict(G=0), b"multiple"),
+    (_scan, dict(n=70000), b"num_seqs"), (_scan, dict(t=-2), b"extents"), (_scan, {}, b"null"),
+    (_scan_step, dict(P=32), b"head_dim"), (_scan_step, dict(b=70000), b"batch"),
+    (_scan_step, {}, b"null"),
+    (_gated, dict(group=48), b"multiple"), (_gated, dict(group=0), b"multiple"),
+    (_gated, dict(act=0), b"activation"), (_gated, dict(eps=-1.0), b"eps"),
+    (_gated, dict(eps=float("nan")), b"eps"), (_gated, dict(dtype=9), b"dtype"),
+    (_gated, {}, b"null"),
+    (_add, dict(width=0), b"width"), (_add, dict(rows=-1), b"rows"), (_add, dict(dtype=-1), b"dtype"),
+    (_add, dict(eps=-1.0), b"eps"), (_add, {}, b"null"),
+])
+def test_c_entry_refuses(fn, kw, word):
+    lib = _lib.load()
+    assert fn(lib, **kw) == BAD
+    assert word in lib.gdn_b200_last_error()
+
+
+@pytest.mark.parametrize("fn,kw", [(_conv, dict(n=0)), (_conv_step, dict(b=0)), (_scan, dict(n=0)),
+                                   (_scan_step, dict(b=0)), (_gated, dict(rows=0)),
+                                   (_add, dict(rows=0))])
+def test_nothing_to_do_is_no_error(fn, kw):
+    lib = _lib.load()
+    assert fn(lib, **kw) == _lib.GDN_B200_OK
+    assert lib.gdn_b200_last_error() == b""
+
+
+def test_python_refuses_cpu_tensors():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w = torch.zeros(64, 4, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    for call in (lambda: M.gdn_short_conv(x, w, None, None, cu, x, None),
+                 lambda: M.gdn_short_conv_step(x, w, None, x, None, x),
+                 lambda: M.gdn_ssm_prefill(x, x, None, x, x, None, None, None, cu, x, x),
+                 lambda: M.gdn_ssm_step(x, x, None, x, x, None, None, x, None, x),
+                 lambda: M.gdn_gated_norm(x, x, None, x),
+                 lambda: M.gdn_add_norm(x, x, x, x, x)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+@pytest.mark.parametrize("shape,name", [((3, 64), "shape"), ((4, 60), "shape")])
+def test_row_checks_name_the_operand(shape, name):
+    t = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="x: expected shape"):
+        M._rows(t, "x", torch.float32, shape, t.device)
+    with pytest.raises(ValueError, match="x: expected torch.bfloat16"):
+        M._rows(t, "x", torch.bfloat16, (4, 64), t.device)
+    with pytest.raises(ValueError, match="contiguous within a row"):
+        M._rows(t.t(), "x", torch.float32, (64, 4), t.device)
+    assert M._rows(t[:, :60], "x", torch.float32, (4, 60), t.device)[1] == 64
+    assert M._rows(t.view(4, 8, 8)[:, :4], "x", torch.float32, (4, 4, 8), t.device)[1] == 64
+    with pytest.raises(ValueError, match="contiguous within a row"):
+        M._rows(t.view(4, 8, 8)[:, :, :4], "x", torch.float32, (4, 8, 4), t.device)
+
+
+# ------------------------------------------------------------------ the oracle
+def test_oracle_convolution_is_a_causal_conv1d():
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(50, 6, generator=g), torch.randn(6, 4, generator=g)
+    b = torch.randn(6, generator=g)
+    ns = torch.zeros(1, 3, 6)
+    out, pool, _ = O.short_conv(x, w, b, None, [0, 50], ns)
+    want = torch.nn.functional.conv1d(x.t()[None].double(), w[:, None].double(), b.double(),
+                                      padding=3, groups=6)[0, :, :50]
+    torch.testing.assert_close(out, torch.nn.functional.silu(want).t())
+    # two pieces with the carried state are the whole
+    first, p1, _ = O.short_conv(x[:2], w, b, None, [0, 2], ns)
+    second, p2, _ = O.short_conv(x[2:], w, b, p1, [0, 48], ns)
+    torch.testing.assert_close(torch.cat([first, second]), out)
+    assert torch.equal(p2, pool)
+
+
+def test_oracle_scan_is_its_closed_form():
+    """y_t = sum_s exp(sum of log decays over (s, t]) (C_t . B_s) step_s x_s + D x_t."""
+    g = torch.Generator().manual_seed(1)
+    T, H, P, G, N = 20, 4, 3, 2, 5
+    x, dt = torch.randn(T, H, P, generator=g), torch.randn(T, H, generator=g)
+    B, C = torch.randn(T, G, N, generator=g), torch.randn(T, G, N, generator=g)
+    A_log, D, bias = (torch.randn(H, generator=g) for _ in range(3))
+    ns = torch.zeros(1, H, P, N)
+    out, pool, mag, pmag = O.scan(x, dt, A_log, B, C, D, bias, None, [0, T], ns)
+    step = torch.nn.functional.softplus(dt.double() + bias)
+    c = (-torch.exp(A_log.double()) * step).cumsum(0)
+    decay = torch.exp(c[:, None] - c[None]).masked_fill(
+        torch.ones(T, T).triu(1).bool()[..., None], 0.0)              # [t, s, H]
+    cb = torch.einsum("tgn,sgn->tsg", C.double(), B.double()).repeat_interleave(2, 2)
+    want = torch.einsum("tsh,tsh,sh,shp->thp", cb, decay, step, x.double())
+    torch.testing.assert_close(out, want + D.double()[:, None] * x)
+    w = torch.exp(c[-1] - c) * step
+    torch.testing.assert_close(pool[0], torch.einsum(
+        "sh,shp,shn->hpn", w, x.double(), B.double().repeat_interleave(2, 1)))
+    assert (mag >= out.abs() - 1e-12).all() and (pmag >= pool.abs() - 1e-12).all()
+
+
+def test_oracle_norms_are_torchs():
+    g = torch.Generator().manual_seed(2)
+    x, z, w = torch.randn(5, 24, generator=g), torch.randn(5, 24, generator=g), torch.randn(24)
+    rms = lambda v, n: torch.nn.functional.rms_norm(v, (n,), eps=1e-6)  # noqa: E731
+    silu = torch.nn.functional.silu(z.double())
+    torch.testing.assert_close(O.gated_norm(x, z, w, 24, 1e-6), rms(x.double(), 24) * w * silu)
+    torch.testing.assert_close(
+        O.gated_norm(x, z, w[:8], 8, 1e-6, norm_first=False),
+        (rms((x * silu).view(5, 3, 8), 8) * w[:8]).view(5, 24))
+    out, r, _ = O.add_norm(x, z, w, scale=0.5, weight_offset=1.0)
+    torch.testing.assert_close(r, z.double() + 0.5 * x)
+    torch.testing.assert_close(out, rms(z.double() + 0.5 * x, 24) * (w + 1.0))
