@@ -64,7 +64,7 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
                          "prefill_split.cuh", "state_affine_kernel.cuh")
     shared = [os.path.join(CSRC, "host_common.h"), os.path.join(INCLUDE, "gdn_b200.h")]
     mixer_deps = _sources("mixer.cu", "gdn_ptx.cuh", "mixer_common.cuh", "short_conv.cuh",
-                          "ssm_recurrent.cuh", "block_norm.cuh")
+                          "ssm_recurrent.cuh", "ssm_scan.cuh", "block_norm.cuh")
     units = [("gdn_b200.cu", core_deps + shared), ("mixer.cu", mixer_deps + shared)]
     objects, stale = [], []
     for src, deps in units:

@@ -177,6 +177,28 @@ int lib_device(unsigned int** status, int* sm_count) noexcept {
   }
 }
 
+int lib_token_map(CUtensorMap* m, const void* base, int width, int heads, long long tokens,
+                  long long stride, int box_tokens) noexcept {
+  try {
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return fail(GDN_B200_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads),
+                          static_cast<cuuint64_t>(tokens)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(width) * 2,
+                             static_cast<cuuint64_t>(stride) * 2};
+    cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_tokens)};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GDN_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    return GDN_B200_OK;
+  } catch (...) {
+    return lib_fail(GDN_B200_ERR_CUDA, "tensor map setup failed");
+  }
+}
+
 }  // namespace gdn
 
 using namespace gdn;

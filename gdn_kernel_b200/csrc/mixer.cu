@@ -6,12 +6,14 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <mutex>
 
 #include "gdn_b200.h"
 #include "host_common.h"
 #include "block_norm.cuh"
 #include "short_conv.cuh"
 #include "ssm_recurrent.cuh"
+#include "ssm_scan.cuh"
 
 namespace gdn {
 namespace {
@@ -171,6 +173,54 @@ int ssm_recurrent_call(const SsmParams& p, int32_t state_dim, int64_t entries, c
   return launched("selective scan launch");
 }
 
+// The scan kernels' shared memory is above the default limit: raised once per
+// device.
+std::mutex g_scan_mu;
+bool g_scan_ready[64];
+
+int scan_setup() {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return lib_cuda_fail(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return lib_fail(GDN_B200_ERR_CUDA, "device index out of range");
+  std::lock_guard<std::mutex> lock(g_scan_mu);
+  if (g_scan_ready[dev]) return GDN_B200_OK;
+  for (auto fn : {gdn_ssm_scan_kernel<64>, gdn_ssm_scan_kernel<128>}) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kScanSmem));
+    if (e != cudaSuccess) return lib_cuda_fail(e, "cudaFuncSetAttribute(scan smem)");
+  }
+  g_scan_ready[dev] = true;
+  return GDN_B200_OK;
+}
+
+int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, cudaStream_t st) {
+  if (int rc = scan_setup()) return rc;
+  // Without tokens every sequence is empty and nothing is loaded; the maps still
+  // need an extent, so they describe one token's worth of new_state.
+  const bool some = p.tokens > 0;
+  CUtensorMap tx, tb, tc;
+  if (int rc = lib_token_map(&tx, some ? static_cast<const void*>(p.x) : p.new_state, p.head_dim,
+                             some ? p.heads : 1, some ? p.tokens : 1,
+                             some ? p.x_stride : p.head_dim, kScanQ))
+    return rc;
+  if (int rc = lib_token_map(&tb, some ? static_cast<const void*>(p.B) : p.new_state, state_dim,
+                             some ? p.groups : 1, some ? p.tokens : 1,
+                             some ? p.b_stride : state_dim, kScanQ))
+    return rc;
+  if (int rc = lib_token_map(&tc, some ? static_cast<const void*>(p.C) : p.new_state, state_dim,
+                             some ? p.groups : 1, some ? p.tokens : 1,
+                             some ? p.c_stride : state_dim, kScanQ))
+    return rc;
+  ScanParams sp;
+  sp.s = p;
+  const dim3 grid(static_cast<unsigned>(p.heads * (p.head_dim / kScanCols)),
+                  static_cast<unsigned>(seqs));
+  if (state_dim == 64) gdn_ssm_scan_kernel<64><<<grid, kScanThreads, kScanSmem, st>>>(tx, tb, tc, sp);
+  else gdn_ssm_scan_kernel<128><<<grid, kScanThreads, kScanSmem, st>>>(tx, tb, tc, sp);
+  return launched("selective scan launch");
+}
+
 }  // namespace
 }  // namespace gdn
 
@@ -282,6 +332,7 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
   if (int rc = check_ssm(total_tokens, pool_size, num_heads, num_groups, head_dim, state_dim))
     return rc;
   if (num_seqs < 0 || num_seqs > 65535) return invalid("num_seqs must be in [0, 65535]");
+  if (total_tokens > kMaxGrid - kScanQ) return invalid("total_tokens exceeds the int32 range");
   if (num_seqs == 0) return GDN_B200_OK;
   if (!cu_seqlens || !new_state) return invalid("null pointer argument");
   if (!state_indices && pool_size < num_seqs)
@@ -322,7 +373,7 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
   if (total_tokens > 0)
     if (int rc = check_ssm_rows(p)) return rc;
   if (int rc = lib_device(&p.status, &sms)) return rc;
-  return ssm_recurrent_call<true>(p, state_dim, num_seqs, static_cast<cudaStream_t>(stream));
+  return ssm_scan_call(p, state_dim, num_seqs, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int gdn_b200_ssm_step(const void* x, int64_t x_stride, const void* dt,
