@@ -20,13 +20,18 @@
 //
 // Decays come from sums towards the chunk's end, sfx_t = L_Q - L_t, which are
 // small and hence accurate exactly where w is not; M and e^L only need the
-// accuracy of bf16.  All exponents are in base 2.
+// accuracy of bf16.  All exponents are in base 2.  M's 32 x 32 blocks below the
+// diagonal ones need no exponential per element: with r the last token of the
+// columns' block, L_t - L_s = (L_t - L_r) + (L_r - L_s), neither part positive,
+// so e^{L_t - L_s} step_s is a row factor times a column factor.
 //
 // Sixteen warps with one role each, handing over through mbarriers:
 //   0 TMA, two stages of {C, B, X}       1 issues the products
-//   2 gates: sfx and log2 step           4-7 S -> M (thread = token row)
+//   2-3 gates: sfx and log2 step         4-7 S -> M (thread = token row)
 //   8-11 w X, and the state in registers (thread = token row / state row)
 //   12-15 outputs (thread = token row)
+// The products of a chunk are issued as dS, Yo, Yd, then S of the next chunk:
+// while Yo, Yd and S run, w X of the next chunk is made from this one's end.
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
 // there, so nothing of them (not even a NaN) enters a product's sum.
 #pragma once
@@ -49,12 +54,23 @@ constexpr uint32_t kScC = 0, kScB = 2 * kScanTile, kScX = 4 * kScanTile;
 constexpr uint32_t kScStage = 5 * kScanTile;
 constexpr uint32_t kScXw = 2 * kScStage;
 constexpr uint32_t kScH = kScXw + 3 * kScanTile;
-constexpr uint32_t kScGate = kScH + kScanTile;            // per stage: g[128], sfx[128]
-constexpr uint32_t kScMisc = kScGate + 2 * 1024;
-constexpr uint32_t kScanSmem = kScMisc + 256;
+constexpr uint32_t kScGate = kScH + kScanTile;   // per stage: g[128], sfx[128], v[96] floats
+constexpr uint32_t kScGateStage = (2 * kScanQ + 96) * 4;
+constexpr uint32_t kScMisc = kScGate + 2 * kScGateStage;
+constexpr uint32_t kScanSmem = kScMisc + 256;    // 227 KiB: all there is
 
 // Tensor memory columns.
 constexpr uint32_t kTmS = 0, kTmM = 128, kTmYd = 192, kTmYo = 256, kTmDs = 320;
+
+// Registers per thread of the four warpgroups: together the 512 x 128 that the
+// block is launched with.
+constexpr int kScanRegs[4] = {72, 104, 208, 128};
+static_assert(kScanRegs[0] + kScanRegs[1] + kScanRegs[2] + kScanRegs[3] == 4 * 128, "as launched");
+
+template <int kRegs> __device__ __forceinline__ void scan_set_regs() {
+  if constexpr (kRegs > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else if constexpr (kRegs < 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 
 // 2^v; 0 for -inf (and for results below the normal range).
 __device__ __forceinline__ float scan_exp2(float v) {
@@ -63,9 +79,53 @@ __device__ __forceinline__ float scan_exp2(float v) {
   return r;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_pair(uint64_t v) {
+  const float2 f = unpair(v);
+  return pack_bf16x2(f.x, f.y);
+}
+// Two packed bf16 as fp32.
+__device__ __forceinline__ uint64_t unpack_pair(uint32_t u) {
+  return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+// The leading 8 bits of both significands as packed bf16, and what is left of
+// the values: exact.  Three of these hold an fp32 value whole.
+__device__ __forceinline__ uint32_t split_pair(uint64_t& v) {
+  const float2 f = unpair(v);
+  const uint32_t x = __float_as_uint(f.x), y = __float_as_uint(f.y);
+  v = fma2(pair(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u)),
+           pair(-1.0f, -1.0f), v);
+  return __byte_perm(x, y, 0x7632);
+}
+
 enum ScanBar {
-  kBFull = 0, kBEmpty = 2, kBGateFull = 4, kBGateEmpty = 6, kBSFull = 8, kBSEmpty, kBMFull,
-  kBYFull, kBYEmpty, kBXwFull, kBDsFull, kBHFull, kBHEmpty, kBDrain, kBCount
+  kBFullX = 0, kBFullBC = 2, kBEmpty = 4, kBEmptyC0 = 6, kBGateFull = 8, kBGateEmpty = 10,
+  kBSFull = 12, kBMFull, kBYFull, kBYEmpty, kBXwFull, kBDsFull, kBHFull, kBHEmpty, kBDrain, kBCount
 };
 
 struct ScanParams {
@@ -120,9 +180,11 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     *abort_flag = 0;
     for (int i = 0; i < kBCount; ++i) {
       int n = 1;
-      if (i == kBEmpty || i == kBEmpty + 1) n = 1 + 4;                // products, output warps
+      if (i == kBEmpty || i == kBEmpty + 1) n = 1 + 4;   // products, output warps
       else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 12;
-      else if (i == kBSEmpty || i == kBMFull || i == kBYEmpty || i == kBXwFull || i == kBHFull) n = 4;
+      else if (i == kBEmptyC0 || i == kBEmptyC0 + 1 || i == kBMFull || i == kBYEmpty ||
+               i == kBXwFull || i == kBHFull)
+        n = 4;
       mbar_init(bars + i, n);
     }
     fence_mbarrier_init();
@@ -150,135 +212,167 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   auto chunk_len = [&](int c) { return min(kScanQ, len - c * kScanQ); };
   constexpr int kSteps = N / 16;   // k-steps over the state dimension
 
-  if (warp == 0) {
-    // ------------------------------------------------ TMA
-    int issued = 0;
-    bool ok = true;
-    for (int c = 0; c < nch; ++c) {
-      const int st = c & 1;
-      if (c >= 2 && !(ok = wait(kBEmpty + st, (c >> 1) - 1, kStatusMmaTimeout))) break;
-      if (elect_one()) {
+  if (warp < 4) {
+    scan_set_regs<kScanRegs[0]>();
+    if (warp == 0) {
+      // ---------------------------------------------- TMA
+      // C's first half is the last part of a stage to come free: the outputs
+      // pass through it.
+      int issued = 0;
+      bool ok = true;
+      for (int c = 0; c < nch; ++c) {
+        const int st = c & 1;
         uint8_t* stage = smem + st * kScStage;
-        uint64_t* bar = bars + kBFull + st;
         const int t0 = static_cast<int>(t_begin) + c * kScanQ;
-        mbar_arrive_expect_tx(bar, (1 + 2 * (N / 64)) * kScanTile);
+        if (c >= 2 && !(ok = wait(kBEmpty + st, (c >> 1) - 1, kStatusMmaTimeout))) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bars + kBFullX + st, kScanTile);
+          tma_load_3d(stage + kScX, &tm_x, bars + kBFullX + st, col0, head, t0);
+          uint64_t* bar = bars + kBFullBC + st;
+          mbar_arrive_expect_tx(bar, 2 * (N / 64) * kScanTile);
 #pragma unroll
-        for (int b = 0; b < N / 64; ++b) {
-          tma_load_3d(stage + kScC + b * kScanTile, &tm_c, bar, 64 * b, group, t0);
-          tma_load_3d(stage + kScB + b * kScanTile, &tm_b, bar, 64 * b, group, t0);
+          for (int b = 0; b < N / 64; ++b)
+            tma_load_3d(stage + kScB + b * kScanTile, &tm_b, bar, 64 * b, group, t0);
+          if constexpr (N == 128) tma_load_3d(stage + kScC + kScanTile, &tm_c, bar, 64, group, t0);
         }
-        tma_load_3d(stage + kScX, &tm_x, bar, col0, head, t0);
+        __syncwarp();
+        issued = c + 1;
+        if (c >= 2) ok = wait(kBEmptyC0 + st, (c >> 1) - 1, kStatusMmaTimeout);
+        if (elect_one()) tma_load_3d(stage + kScC, &tm_c, bars + kBFullBC + st, 0, group, t0);
+        __syncwarp();
+        if (!ok) break;
       }
-      __syncwarp();
-      issued = c + 1;
-    }
-    if (!ok)   // aborted: the copies in flight land first
-      for (int c = max(issued - 2, 0); c < issued; ++c) mbar_wait(bars + kBFull + (c & 1), (c >> 1) & 1);
-  } else if (warp == 1) {
-    // ------------------------------------------------ products
-    constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, 0, 0);
-    constexpr uint32_t idesc_y = idesc_bf16_f32(128, 64, 0, 1);
-    constexpr uint32_t idesc_ds = idesc_bf16_f32(128, 192, 1, 1);
-    const uint32_t base = smem_u32(smem);
-    auto issue_s = [&](int c) {
-      const uint32_t st = base + (c & 1) * kScStage;
-      if (elect_one()) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const uint32_t off = (s >> 2) * kScanTile + (s & 3) * 32;
-          umma_bf16(tmem + kTmS, sdesc_sw128(st + kScC + off, 16, 1024),
-                    sdesc_sw128(st + kScB + off, 16, 1024), idesc_s, s > 0);
+      if (!ok)   // aborted: the copies in flight land first
+        for (int c = max(issued - 2, 0); c < issued; ++c) {
+          mbar_wait(bars + kBFullX + (c & 1), (c >> 1) & 1);
+          mbar_wait(bars + kBFullBC + (c & 1), (c >> 1) & 1);
         }
-        umma_commit(bars + kBSFull);
-      }
-      __syncwarp();
-    };
-    bool ok = wait(kBFull, 0, kStatusTmaTimeout);
-    if (ok) issue_s(0);
-    for (int c = 0; ok && c < nch; ++c) {
-      const uint32_t st = base + (c & 1) * kScStage;
-      const int ksteps = (chunk_len(c) + 15) / 16;
-      if (!(ok = wait(kBXwFull, c, kStatusMmaTimeout))) break;
-      tc_fence_after();
-      if (elect_one()) {
-        for (int s = 0; s < ksteps; ++s)
-          umma_bf16(tmem + kTmDs, sdesc_sw128(st + kScB + s * 2048, kScanTile, 1024),
-                    sdesc_sw128(base + kScXw + s * 2048, kScanTile, 1024), idesc_ds, s > 0);
-        umma_commit(bars + kBDsFull);
-      }
-      __syncwarp();
-      if (!(ok = wait(kBHFull, c, kStatusMmaTimeout))) break;
-      if (c > 0 && !(ok = wait(kBYEmpty, c - 1, kStatusMmaTimeout))) break;
-      tc_fence_after();
-      if (elect_one()) {
+    } else if (warp == 1) {
+      // ---------------------------------------------- products
+      constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, 0, 0);
+      constexpr uint32_t idesc_y = idesc_bf16_f32(128, 64, 0, 1);
+      constexpr uint32_t idesc_ds = idesc_bf16_f32(128, 192, 1, 1);
+      const uint32_t base = smem_u32(smem);
+      auto issue_s = [&](int c) {
+        const uint32_t st = base + (c & 1) * kScStage;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-          umma_bf16(tmem + kTmYo,
-                    sdesc_sw128(st + kScC + (s >> 2) * kScanTile + (s & 3) * 32, 16, 1024),
-                    sdesc_sw128(base + kScH + s * 2048, kScanTile, 1024), idesc_y, s > 0);
-        umma_commit(bars + kBHEmpty);
-      }
-      __syncwarp();
-      if (c + 1 < nch) {
-        if (!(ok = wait(kBFull + ((c + 1) & 1), (c + 1) >> 1, kStatusTmaTimeout))) break;
-        if (!(ok = wait(kBSEmpty, c, kStatusMmaTimeout))) break;
+          for (int s = 0; s < kSteps; ++s) {
+            const uint32_t off = (s >> 2) * kScanTile + (s & 3) * 32;
+            umma_bf16(tmem + kTmS, sdesc_sw128(st + kScC + off, 16, 1024),
+                      sdesc_sw128(st + kScB + off, 16, 1024), idesc_s, s > 0);
+          }
+          umma_commit(bars + kBSFull);
+        }
+        __syncwarp();
+      };
+      bool ok = wait(kBFullBC, 0, kStatusTmaTimeout);
+      if (ok) issue_s(0);
+      for (int c = 0; ok && c < nch; ++c) {
+        const uint32_t st = base + (c & 1) * kScStage;
+        const int ksteps = (chunk_len(c) + 15) / 16;
+        if (!(ok = wait(kBXwFull, c, kStatusMmaTimeout))) break;
         tc_fence_after();
-        issue_s(c + 1);
-      }
-      if (!(ok = wait(kBMFull, c, kStatusMmaTimeout))) break;
-      tc_fence_after();
-      if (elect_one()) {
-        for (int s = 0; s < ksteps; ++s)
-          umma_bf16_ts(tmem + kTmYd, tmem + kTmM + s * 8,
-                       sdesc_sw128(st + kScX + s * 2048, kScanTile, 1024), idesc_y, s > 0);
-        umma_commit(bars + kBYFull);
-        if (c + 2 < nch) umma_commit(bars + kBEmpty + (c & 1));
-      }
-      __syncwarp();
-    }
-    if (!ok) {   // aborted: the products in flight finish first
-      if (elect_one()) umma_commit(bars + kBDrain);
-      __syncwarp();
-      mbar_wait(bars + kBDrain, 0);
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------ gates
-    const float a2 = -expf(p.A_log[head]) * 1.4426950408889634f;
-    const float bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
-    const __nv_bfloat16* dt = p.dt + head;
-    for (int c = 0; c < nch; ++c) {
-      const int st = c & 1, n = chunk_len(c);
-      const long long t0 = t_begin + static_cast<long long>(c) * kScanQ;
-      float step[4], la[4];
+        if (elect_one()) {
+          for (int s = 0; s < ksteps; ++s)
+            umma_bf16(tmem + kTmDs, sdesc_sw128(st + kScB + s * 2048, kScanTile, 1024),
+                      sdesc_sw128(base + kScXw + s * 2048, kScanTile, 1024), idesc_ds, s > 0);
+          umma_commit(bars + kBDsFull);
+        }
+        __syncwarp();
+        if (!(ok = wait(kBHFull, c, kStatusMmaTimeout))) break;
+        if (c > 0 && !(ok = wait(kBYEmpty, c - 1, kStatusMmaTimeout))) break;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 4 * lane + i;
-        step[i] = t < n ? ssm_step_size(to_float(dt[(t0 + t) * p.dt_stride]) + bias) : 0.0f;
-        la[i] = a2 * step[i];
+          for (int s = 0; s < kSteps; ++s)
+            umma_bf16(tmem + kTmYo,
+                      sdesc_sw128(st + kScC + (s >> 2) * kScanTile + (s & 3) * 32, 16, 1024),
+                      sdesc_sw128(base + kScH + s * 2048, kScanTile, 1024), idesc_y, s > 0);
+          umma_commit(bars + kBHEmpty);
+        }
+        __syncwarp();
+        if (!(ok = wait(kBMFull, c, kStatusMmaTimeout))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          for (int s = 0; s < ksteps; ++s)
+            umma_bf16_ts(tmem + kTmYd, tmem + kTmM + s * 8,
+                         sdesc_sw128(st + kScX + s * 2048, kScanTile, 1024), idesc_y, s > 0);
+          umma_commit(bars + kBYFull);
+          if (c + 2 < nch) umma_commit(bars + kBEmpty + (c & 1));
+        }
+        __syncwarp();
+        if (c + 1 < nch) {   // M of this chunk is made, so S is read
+          if (!(ok = wait(kBFullBC + ((c + 1) & 1), (c + 1) >> 1, kStatusTmaTimeout))) break;
+          issue_s(c + 1);
+        }
       }
-      float s3 = 0.0f, s2 = la[3], s1 = s2 + la[2], s0 = s1 + la[1];
-      const float mine = s0 + la[0];
-      float v = mine;   // sums over this lane and those after it
+      if (!ok) {   // aborted: the products in flight finish first
+        if (elect_one()) umma_commit(bars + kBDrain);
+        __syncwarp();
+        mbar_wait(bars + kBDrain, 0);
+      }
+    } else {
+      // ---------------------------------------------- gates
+      // Two warps take turns; a chunk's dt are on their way while the chunk
+      // before it (of this warp) is worked on.
+      const float a2 = -expf(p.A_log[head]) * 1.4426950408889634f;
+      const float bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
+      const __nv_bfloat16* dt = p.dt + t_begin * p.dt_stride + head;
+      __nv_bfloat16 raw[4];
+      auto load_dt = [&](int c) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float u = __shfl_down_sync(0xffffffffu, v, o);
-        if (lane + o < 32) v += u;
+        for (int i = 0; i < 4; ++i) {
+          const int t = c * kScanQ + 4 * lane + i;
+          raw[i] = __float2bfloat16_rn(0.0f);
+          if (t < len) raw[i] = dt[t * p.dt_stride];
+        }
+      };
+      load_dt(warp - 2);
+      for (int c = warp - 2; c < nch; c += 2) {
+        const int st = c & 1, n = chunk_len(c);
+        float step[4], la[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          step[i] = 4 * lane + i < n ? ssm_step_size(to_float(raw[i]) + bias) : 0.0f;
+          la[i] = a2 * step[i];
+        }
+        load_dt(c + 2);
+        float sfx[4];
+        sfx[3] = 0.0f;
+        sfx[2] = la[3];
+        sfx[1] = sfx[2] + la[2];
+        sfx[0] = sfx[1] + la[1];
+        float v = sfx[0] + la[0];   // sums over this lane and those after it
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float u = __shfl_down_sync(0xffffffffu, v, o);
+          if (lane + o < 32) v += u;
+        }
+        float after = __shfl_down_sync(0xffffffffu, v, 1);
+        if (lane == 31) after = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sfx[i] += after;
+        // the last token of this lane's 32
+        const float ref = __shfl_sync(0xffffffffu, sfx[3], lane | 7);
+        if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) break;
+        float* g = reinterpret_cast<float*>(smem + kScGate + st * kScGateStage);
+        reinterpret_cast<float4*>(g + kScanQ)[lane] = make_float4(sfx[0], sfx[1], sfx[2], sfx[3]);
+        // log2 of a zero step is -inf: a padded token has no weight anywhere
+        reinterpret_cast<float4*>(g)[lane] =
+            make_float4(sfx[0] + log2f(step[0]), sfx[1] + log2f(step[1]), sfx[2] + log2f(step[2]),
+                        sfx[3] + log2f(step[3]));
+        if (lane < 24)
+          reinterpret_cast<float4*>(g + 2 * kScanQ)[lane] =
+              make_float4(step[0] * scan_exp2(sfx[0] - ref), step[1] * scan_exp2(sfx[1] - ref),
+                          step[2] * scan_exp2(sfx[2] - ref), step[3] * scan_exp2(sfx[3] - ref));
+        if (lane == 0) totals[st] = v;
+        arrive(kBGateFull + st);
       }
-      float after = __shfl_down_sync(0xffffffffu, v, 1);
-      if (lane == 31) after = 0.0f;
-      if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) break;
-      float* g = reinterpret_cast<float*>(smem + kScGate + st * 1024);
-      const float4 sfx = make_float4(after + s0, after + s1, after + s2, after + s3);
-      reinterpret_cast<float4*>(g + kScanQ)[lane] = sfx;
-      // log2 of a zero step is -inf: a padded token has no weight anywhere
-      reinterpret_cast<float4*>(g)[lane] =
-          make_float4(sfx.x + log2f(step[0]), sfx.y + log2f(step[1]), sfx.z + log2f(step[2]),
-                      sfx.w + log2f(step[3]));
-      if (lane == 0) totals[st] = v;
-      arrive(kBGateFull + st);
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp < 8) {
     // ------------------------------------------------ S -> M
+    scan_set_regs<kScanRegs[1]>();
     {   // blocks above the diagonal stay zero
       const uint32_t z[16] = {};
       for (int b = quad + 1; b < 4; ++b) tmem_st16(tmem + kTmM + 16 * b + tm_lane, z);
@@ -287,113 +381,137 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     for (int c = 0; c < nch; ++c) {
       const int st = c & 1;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
-      if (!wait(kBSFull, c, kStatusMmaTimeout)) break;
-      if (c > 0 && !wait(kBYFull, c - 1, kStatusMmaTimeout)) break;   // the last M is read
-      tc_fence_after();
-      const float* g = reinterpret_cast<const float*>(smem + kScGate + st * 1024);
+      const float* g = reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage);
       const float mine = g[kScanQ + row];
-      for (int b = 0; b <= quad; ++b) {
+      if (!wait(kBSFull, c, kStatusMmaTimeout)) break;   // also: the last M is read
+      tc_fence_after();
+      for (int b = 0; b < quad; ++b) {
         float s[32];
         tmem_ld32(tmem + kTmS + 32 * b + tm_lane, s);
-        tmem_wait_ld();
+        const float u = scan_exp2(g[kScanQ + 32 * b + 31] - mine);
+        const uint64_t u2 = pair(u, u);
+        const float4* v = reinterpret_cast<const float4*>(g + 2 * kScanQ + 32 * b);
         uint32_t m[16];
+        tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float4 gv = *reinterpret_cast<const float4*>(g + 32 * b + 4 * j);
+          const float4 f = v[j];
+          m[2 * j] = pack_pair(mul2(mul2(pair(s[4 * j], s[4 * j + 1]), u2), pair(f.x, f.y)));
+          m[2 * j + 1] = pack_pair(mul2(mul2(pair(s[4 * j + 2], s[4 * j + 3]), u2), pair(f.z, f.w)));
+        }
+        tmem_st16(tmem + kTmM + 16 * b + tm_lane, m);
+      }
+      {
+        float s[32];
+        tmem_ld32(tmem + kTmS + 32 * quad + tm_lane, s);
+        const float4* f4 = reinterpret_cast<const float4*>(g + 32 * quad);
+        uint32_t m[16];
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 gv = f4[j];
           const float f[4] = {gv.x, gv.y, gv.z, gv.w};
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)   // a select: a masked S may hold anything
-            v[e] = 32 * b + 4 * j + e <= row ? s[4 * j + e] * scan_exp2(f[e] - mine) : 0.0f;
+            v[e] = 4 * j + e <= lane ? s[4 * j + e] * scan_exp2(f[e] - mine) : 0.0f;
           m[2 * j] = pack_bf16x2(v[0], v[1]);
           m[2 * j + 1] = pack_bf16x2(v[2], v[3]);
         }
-        tmem_st16(tmem + kTmM + 16 * b + tm_lane, m);
+        tmem_st16(tmem + kTmM + 16 * quad + tm_lane, m);
       }
       tmem_wait_st();
       tc_fence_before();
-      arrive(kBSEmpty);
       arrive(kBMFull);
       arrive(kBGateEmpty + st);
     }
-  } else if (warp >= 8 && warp < 12) {
+  } else if (warp < 12) {
     // ------------------------------------------------ w X and the state
+    scan_set_regs<kScanRegs[2]>();
     const bool state_row = row < N;
-    float h[kScanCols];
+    uint64_t h[kScanCols / 2];
 #pragma unroll
-    for (int j = 0; j < kScanCols; ++j)
-      h[j] = carried && state_row ? p.state[sbase + static_cast<long long>(j) * N + row] : 0.0f;
+    for (int j = 0; j < kScanCols / 2; ++j) {
+      const float* src = p.state + sbase + static_cast<long long>(2 * j) * N + row;
+      const bool read = carried && state_row;
+      h[j] = pair(read ? src[0] : 0.0f, read ? src[N] : 0.0f);
+    }
     auto add_ds = [&](float decay) {
+      const uint64_t d2 = pair(decay, decay);
 #pragma unroll
-      for (int j = 0; j < kScanCols; ++j) h[j] *= decay;
+      for (int b = 0; b < 2; ++b) {
+        float d[3][32];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+        for (int k = 0; k < 3; ++k) tmem_ld32(tmem + kTmDs + 64 * k + 32 * b + tm_lane, d[k]);
+        tmem_wait_ld();
 #pragma unroll
-        for (int k = 2; k >= 0; --k) {   // the small parts first
-          float d[32];
-          tmem_ld32(tmem + kTmDs + 64 * k + 32 * b + tm_lane, d);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) h[32 * b + j] += d[j];
+        for (int j = 0; j < 16; ++j) {   // the small parts first
+          const uint64_t t = add2(add2(pair(d[2][2 * j], d[2][2 * j + 1]),
+                                       pair(d[1][2 * j], d[1][2 * j + 1])),
+                                  pair(d[0][2 * j], d[0][2 * j + 1]));
+          h[16 * b + j] = fma2(h[16 * b + j], d2, t);
         }
+      }
     };
     bool ok = true;
     float decay = 1.0f;
     for (int c = 0; c < nch; ++c) {
       const int st = c & 1, n = chunk_len(c);
       uint8_t* stage = smem + st * kScStage;
+      if (!(ok = wait(kBGateFull + st, c >> 1, kStatusMmaTimeout))) break;
+      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[row]);
+      const float next_decay = scan_exp2(totals[st]);
+      arrive(kBGateEmpty + st);
       if (c > 0) {
         if (!(ok = wait(kBDsFull, c - 1, kStatusMmaTimeout))) break;
         tc_fence_after();
         add_ds(decay);
         tc_fence_before();
       }
-      if (!(ok = wait(kBGateFull + st, c >> 1, kStatusMmaTimeout))) break;
-      if (!(ok = wait(kBFull + st, c >> 1, kStatusTmaTimeout))) break;
-      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kScGate + st * 1024)[row]);
-      decay = scan_exp2(totals[st]);
-      const bool past = row >= n;
+      decay = next_decay;
+      if (!(ok = wait(kBFullX + st, c >> 1, kStatusTmaTimeout))) break;
+      if (n < kScanQ) {   // a last, short chunk: what lies past it must not count
+        if (!(ok = wait(kBFullBC + st, c >> 1, kStatusTmaTimeout))) break;
+        if (row >= n) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t off = sw128_off(row, j);
+            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(stage + kScX + off) = z;
+#pragma unroll
+            for (int b = 0; b < N / 64; ++b)
+              *reinterpret_cast<uint4*>(stage + kScB + b * kScanTile + off) = z;
+          }
+        }
+      }
+      const uint64_t w2 = pair(w, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t off = sw128_off(row, j);
-        uint4 u = *reinterpret_cast<const uint4*>(stage + kScX + off);
-        if (past) u = make_uint4(0u, 0u, 0u, 0u);
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + kScX + off);
         const uint32_t in[4] = {u.x, u.y, u.z, u.w};
         uint32_t part[3][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&in[i]));
-          v.x *= past ? 0.0f : w;
-          v.y *= past ? 0.0f : w;
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            part[k][i] = pack_bf16x2(v.x, v.y);
-            const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&part[k][i]));
-            v.x -= r.x;
-            v.y -= r.y;
-          }
+          uint64_t v = mul2(unpack_pair(in[i]), w2);
+          part[0][i] = split_pair(v);
+          part[1][i] = split_pair(v);
+          part[2][i] = pack_pair(v);
         }
 #pragma unroll
         for (int k = 0; k < 3; ++k)
           *reinterpret_cast<uint4*>(smem + kScXw + k * kScanTile + off) =
               make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
-        if (past) {
-          *reinterpret_cast<uint4*>(stage + kScX + off) = u;
-#pragma unroll
-          for (int b = 0; b < N / 64; ++b)
-            *reinterpret_cast<uint4*>(stage + kScB + b * kScanTile + off) = u;
-        }
       }
       fence_proxy_async_smem();
       arrive(kBXwFull);
-      arrive(kBGateEmpty + st);
       if (c > 0 && !(ok = wait(kBHEmpty, c - 1, kStatusMmaTimeout))) break;
       if (state_row) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           *reinterpret_cast<uint4*>(smem + kScH + sw128_off(row, j)) =
-              make_uint4(pack_bf16x2(h[8 * j], h[8 * j + 1]), pack_bf16x2(h[8 * j + 2], h[8 * j + 3]),
-                         pack_bf16x2(h[8 * j + 4], h[8 * j + 5]), pack_bf16x2(h[8 * j + 6], h[8 * j + 7]));
+              make_uint4(pack_pair(h[4 * j]), pack_pair(h[4 * j + 1]), pack_pair(h[4 * j + 2]),
+                         pack_pair(h[4 * j + 3]));
       }
       fence_proxy_async_smem();
       arrive(kBHFull);
@@ -404,58 +522,73 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       tc_fence_before();
       if (slot >= 0 && state_row) {
 #pragma unroll
-        for (int j = 0; j < kScanCols; ++j)
-          p.new_state[sbase + static_cast<long long>(j) * N + row] = h[j];
+        for (int j = 0; j < kScanCols / 2; ++j) {
+          float* dst = p.new_state + sbase + static_cast<long long>(2 * j) * N + row;
+          const float2 f = unpair(h[j]);
+          dst[0] = f.x;
+          dst[N] = f.y;
+        }
       }
     }
-  } else if (warp >= 12) {
+  } else {
     // ------------------------------------------------ outputs
+    scan_set_regs<kScanRegs[3]>();
     const float D = p.D ? p.D[head] : 0.0f;
+    const uint64_t D2 = pair(D, D);
     for (int c = 0; c < nch; ++c) {
       const int st = c & 1, n = chunk_len(c);
-      uint8_t* x = smem + st * kScStage + kScX;
+      uint8_t* stage = smem + st * kScStage;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
-      const float e = scan_exp2(totals[st] - reinterpret_cast<const float*>(smem + kScGate + st * 1024)[kScanQ + row]);
+      const float e = scan_exp2(
+          totals[st] - reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row]);
       arrive(kBGateEmpty + st);
+      if (!wait(kBFullX + st, c >> 1, kStatusTmaTimeout)) break;
+      uint4 x[8];   // kept here so that the stage can be refilled early
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x[j] = *reinterpret_cast<const uint4*>(stage + kScX + sw128_off(row, j));
+      arrive(kBEmpty + st);
       if (!wait(kBYFull, c, kStatusMmaTimeout)) break;
       tc_fence_after();
-      // the row's results take the place of its X in shared memory (no product
-      // reads it any more), and the warp writes whole rows from there
+      // the row's results go to C's first half in shared memory (no product
+      // reads it any more), from where the warp writes whole rows
+      const uint64_t e2 = pair(e, e);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         float yd[32], yo[32];
         tmem_ld32(tmem + kTmYd + 32 * b + tm_lane, yd);
         tmem_ld32(tmem + kTmYo + 32 * b + tm_lane, yo);
         tmem_wait_ld();
+        if (b == 1) {
+          tc_fence_before();
+          arrive(kBYEmpty);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t off = sw128_off(row, 4 * b + j);
-          const uint4 u = *reinterpret_cast<const uint4*>(x + off);
-          const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+          const uint32_t in[4] = {x[4 * b + j].x, x[4 * b + j].y, x[4 * b + j].z, x[4 * b + j].w};
           uint32_t out[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&in[i]));
             const int k = 8 * j + 2 * i;
-            out[i] = pack_bf16x2(fmaf(D, v.x, fmaf(e, yo[k], yd[k])),
-                                 fmaf(D, v.y, fmaf(e, yo[k + 1], yd[k + 1])));
+            out[i] = pack_pair(fma2(D2, unpack_pair(in[i]),
+                                    fma2(e2, pair(yo[k], yo[k + 1]), pair(yd[k], yd[k + 1]))));
           }
-          *reinterpret_cast<uint4*>(x + off) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(stage + kScC + sw128_off(row, 4 * b + j)) =
+              make_uint4(out[0], out[1], out[2], out[3]);
         }
       }
-      tc_fence_before();
-      arrive(kBYEmpty);
+      __syncwarp();
       __nv_bfloat16* out = p.out +
           ((t_begin + static_cast<long long>(c) * kScanQ) * p.heads + head) * p.head_dim + col0;
       const long long ld = static_cast<long long>(p.heads) * p.head_dim;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = quad * 32 + 4 * i + (lane >> 3);
-        const uint4 u = *reinterpret_cast<const uint4*>(x + sw128_off(r, lane & 7));
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + kScC + sw128_off(r, lane & 7));
         if (r < n) *reinterpret_cast<uint4*>(out + r * ld + 8 * (lane & 7)) = u;
       }
-      fence_proxy_async_smem();   // the next copy into this stage comes after these accesses
-      arrive(kBEmpty + st);
+      fence_proxy_async_smem();   // the next copy into this half comes after these accesses
+      arrive(kBEmptyC0 + st);
     }
   }
   tc_fence_before();
