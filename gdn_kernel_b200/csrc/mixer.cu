@@ -190,12 +190,51 @@ int scan_setup() {
                              static_cast<int>(kScanSmem));
     if (e != cudaSuccess) return lib_cuda_fail(e, "cudaFuncSetAttribute(scan smem)");
   }
+  for (auto fn : {gdn_ssm_piece_state_kernel<64>, gdn_ssm_piece_state_kernel<128>}) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kStateSmem));
+    if (e != cudaSuccess) return lib_cuda_fail(e, "cudaFuncSetAttribute(piece state smem)");
+  }
   g_scan_ready[dev] = true;
   return GDN_B200_OK;
 }
 
-int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, cudaStream_t st) {
+// How a call's sequences are divided.  A CTA runs 64 columns of a head; with
+// fewer (sequence, CTA) pairs than keep the SMs busy, long sequences run in
+// pieces.  Pieces of 1 / (2 SMs) of all chunks leave two or three CTAs to each
+// SM, enough to even out; below kScanMinPiece chunks a piece costs more in
+// starting up than it saves.
+constexpr int kScanPiecesPerSm = 1;
+constexpr int kScanSms = 148, kScanMinPiece = 4, kScanMaxDivided = 1024;
+
+struct ScanPlan {
+  int seg_chunks;        // 0: not divided
+  long long max_full;    // bound on the whole pieces
+  size_t state_bytes, bytes;
+};
+
+ScanPlan scan_plan(long long seqs, long long tokens, int heads, int head_dim, int state_dim) {
+  ScanPlan plan{};
+  const long long chunks = tokens / kScanQ + seqs;   // no fewer than there are
+  const long long units = static_cast<long long>(heads) * (head_dim / kScanCols);
+  if (seqs > kScanMaxDivided || seqs * units >= 8 * kScanSms) return plan;
+  const long long piece =
+      std::max<long long>(kScanMinPiece, (tokens / kScanQ * units + kScanPiecesPerSm * kScanSms - 1) / (kScanPiecesPerSm * kScanSms));
+  if (tokens / kScanQ < piece) return plan;
+  plan.seg_chunks = static_cast<int>(piece);
+  plan.max_full = chunks / piece;
+  const size_t row = static_cast<size_t>(heads) * head_dim * state_dim * 4;
+  plan.state_bytes = 2 * plan.max_full * row;
+  plan.bytes = plan.state_bytes + plan.max_full * heads * 4;
+  return plan;
+}
+
+int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, void* workspace,
+                  uint64_t workspace_bytes, cudaStream_t st) {
   if (int rc = scan_setup()) return rc;
+  ScanPlan plan = scan_plan(seqs, p.tokens, p.heads, p.head_dim, state_dim);
+  if (!workspace || workspace_bytes < plan.bytes) plan = ScanPlan{};
+  if (plan.max_full + seqs > 65535) plan = ScanPlan{};
   // Without tokens every sequence is empty and nothing is loaded; the maps still
   // need an extent, so they describe one token's worth of new_state.
   const bool some = p.tokens > 0;
@@ -212,10 +251,21 @@ int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, cudaStrea
                              some ? p.groups : 1, some ? p.tokens : 1,
                              some ? p.c_stride : state_dim, kScanQ))
     return rc;
-  ScanParams sp;
+  ScanParams sp{};
   sp.s = p;
-  const dim3 grid(static_cast<unsigned>(p.heads * (p.head_dim / kScanCols)),
-                  static_cast<unsigned>(seqs));
+  sp.seg_chunks = plan.seg_chunks;
+  sp.max_full = static_cast<int>(plan.max_full);
+  sp.seg_state = static_cast<float*>(workspace);
+  sp.seg_decay = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.state_bytes);
+  const unsigned units = static_cast<unsigned>(p.heads * (p.head_dim / kScanCols));
+  if (plan.max_full > 0) {
+    const dim3 pieces(units, static_cast<unsigned>(plan.max_full));
+    if (state_dim == 64)
+      gdn_ssm_piece_state_kernel<64><<<pieces, kStateThreads, kStateSmem, st>>>(tx, tb, sp);
+    else
+      gdn_ssm_piece_state_kernel<128><<<pieces, kStateThreads, kStateSmem, st>>>(tx, tb, sp);
+  }
+  const dim3 grid(units, static_cast<unsigned>(plan.max_full + seqs));
   if (state_dim == 64) gdn_ssm_scan_kernel<64><<<grid, kScanThreads, kScanSmem, st>>>(tx, tb, tc, sp);
   else gdn_ssm_scan_kernel<128><<<grid, kScanThreads, kScanSmem, st>>>(tx, tb, tc, sp);
   return launched("selective scan launch");
@@ -310,9 +360,12 @@ extern "C" int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const v
   return conv_call(p, width, dtype, batch, true, stream);
 }
 
-extern "C" uint64_t gdn_b200_ssm_prefill_workspace_size(int64_t, int64_t, int32_t, int32_t,
-                                                        int32_t) {
-  return 0;
+extern "C" uint64_t gdn_b200_ssm_prefill_workspace_size(int64_t num_seqs, int64_t total_tokens,
+                                                        int32_t num_heads, int32_t head_dim,
+                                                        int32_t state_dim) {
+  if (num_seqs <= 0 || total_tokens <= 0 || num_heads <= 0 || head_dim <= 0 || state_dim <= 0)
+    return 0;
+  return scan_plan(num_seqs, total_tokens, num_heads, head_dim, state_dim).bytes;
 }
 
 extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void* dt,
@@ -327,8 +380,6 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
                                     int32_t state_dim, void* workspace, uint64_t workspace_bytes,
                                     void* stream) {
   lib_clear_error();
-  (void)workspace;
-  (void)workspace_bytes;
   if (int rc = check_ssm(total_tokens, pool_size, num_heads, num_groups, head_dim, state_dim))
     return rc;
   if (num_seqs < 0 || num_seqs > 65535) return invalid("num_seqs must be in [0, 65535]");
@@ -340,6 +391,7 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
   if (!aligned(cu_seqlens, cu_seqlens_is_int64 ? 8 : 4) ||
       !aligned(state_indices, indices_are_int64 ? 8 : 4))
     return invalid("cu_seqlens or state_indices is misaligned");
+  if (!aligned(workspace, 256)) return invalid("workspace needs 256-byte alignment");
   if (!aligned(state, 16) || !aligned(new_state, 16))
     return invalid("state and new_state need 16-byte alignment");
   SsmParams p{};
@@ -373,7 +425,8 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
   if (total_tokens > 0)
     if (int rc = check_ssm_rows(p)) return rc;
   if (int rc = lib_device(&p.status, &sms)) return rc;
-  return ssm_scan_call(p, state_dim, num_seqs, static_cast<cudaStream_t>(stream));
+  return ssm_scan_call(p, state_dim, num_seqs, workspace, workspace_bytes,
+                       static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int gdn_b200_ssm_step(const void* x, int64_t x_stride, const void* dt,

@@ -25,13 +25,13 @@
 // columns' block, L_t - L_s = (L_t - L_r) + (L_r - L_s), neither part positive,
 // so e^{L_t - L_s} step_s is a row factor times a column factor.
 //
-// Sixteen warps with one role each, handing over through mbarriers:
+// Twenty warps with one role each, handing over through mbarriers:
 //   0 TMA, two stages of {C, B, X}       1 issues the products
-//   2-3 gates: sfx and log2 step         4-7 S -> M (thread = token row)
-//   8-11 w X, and the state in registers (thread = token row / state row)
-//   12-15 outputs (thread = token row)
-// The products of a chunk are issued as dS, Yo, Yd, then S of the next chunk:
-// while Yo, Yd and S run, w X of the next chunk is made from this one's end.
+//   4-7 gates, and S -> M (thread = token row)
+//   8-11 the state in registers (thread = state row)
+//   12-15 outputs (thread = token row)   16-19 w X (thread = token row)
+// The products of a chunk are issued as dS, Yo, Yd, then S of the next chunk.
+// The next w X is made in registers while dS still reads the last one.
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
 // there, so nothing of them (not even a NaN) enters a product's sum.
 #pragma once
@@ -45,7 +45,7 @@ namespace gdn {
 
 constexpr int kScanQ = 128;
 constexpr int kScanCols = 64;            // columns of P per CTA
-constexpr int kScanThreads = 512;
+constexpr int kScanThreads = 640;
 constexpr uint32_t kScanTile = 16384;    // 128 rows x 64 bf16
 
 // Shared memory: two stages of C (two halves of N), B (two halves) and X, the
@@ -57,19 +57,23 @@ constexpr uint32_t kScH = kScXw + 3 * kScanTile;
 constexpr uint32_t kScGate = kScH + kScanTile;   // per stage: g[128], sfx[128], v[96] floats
 constexpr uint32_t kScGateStage = (2 * kScanQ + 96) * 4;
 constexpr uint32_t kScMisc = kScGate + 2 * kScGateStage;
-constexpr uint32_t kScanSmem = kScMisc + 256;    // 227 KiB: all there is
+constexpr uint32_t kScItem = kScMisc + 224;       // barriers and flags before it
+constexpr uint32_t kScanSmem = kScMisc + 256;     // 227 KiB: all there is
 
 // Tensor memory columns.
 constexpr uint32_t kTmS = 0, kTmM = 128, kTmYd = 192, kTmYo = 256, kTmDs = 320;
 
-// Registers per thread of the four warpgroups: together the 512 x 128 that the
+// Registers per thread of the five warpgroups: together the 640 x 96 that the
 // block is launched with.
-constexpr int kScanRegs[4] = {72, 104, 208, 128};
-static_assert(kScanRegs[0] + kScanRegs[1] + kScanRegs[2] + kScanRegs[3] == 4 * 128, "as launched");
+constexpr int kScanLaunchRegs = 96;
+constexpr int kScanRegs[5] = {56, 88, 120, 88, 128};
+static_assert(kScanRegs[0] + kScanRegs[1] + kScanRegs[2] + kScanRegs[3] + kScanRegs[4] ==
+                  5 * kScanLaunchRegs && kScanThreads * kScanLaunchRegs <= 65536,
+              "as launched");
 
 template <int kRegs> __device__ __forceinline__ void scan_set_regs() {
-  if constexpr (kRegs > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-  else if constexpr (kRegs < 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+  if constexpr (kRegs > kScanLaunchRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else if constexpr (kRegs < kScanLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 // 2^v; 0 for -inf (and for results below the normal range).
@@ -83,6 +87,11 @@ __device__ __forceinline__ float scan_exp2(float v) {
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_bits(uint32_t x, uint32_t y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
   return r;
 }
 __device__ __forceinline__ float2 unpair(uint64_t v) {
@@ -113,6 +122,11 @@ __device__ __forceinline__ uint32_t pack_pair(uint64_t v) {
 __device__ __forceinline__ uint64_t unpack_pair(uint32_t u) {
   return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
+// A value that every lane holds, so that the compiler knows it: products, copies
+// and their descriptors want uniform registers, and without this each is wrapped
+// in a loop over the lanes' values (50 instructions per product).
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // The leading 8 bits of both significands as packed bf16, and what is left of
 // the values: exact.  Three of these hold an fp32 value whole.
 __device__ __forceinline__ uint32_t split_pair(uint64_t& v) {
@@ -125,12 +139,436 @@ __device__ __forceinline__ uint32_t split_pair(uint64_t& v) {
 
 enum ScanBar {
   kBFullX = 0, kBFullBC = 2, kBEmpty = 4, kBEmptyC0 = 6, kBGateFull = 8, kBGateEmpty = 10,
-  kBSFull = 12, kBMFull, kBYFull, kBYEmpty, kBXwFull, kBDsFull, kBHFull, kBHEmpty, kBDrain, kBCount
+  kBSFull = 12, kBMFull, kBYFull, kBYEmpty, kBXwFull, kBDsFull, kBDsEmpty, kBHFull, kBHEmpty,
+  kBGateSum, kBDrain, kBCount
 };
 
+// Long sequences run in pieces of seg_chunks chunks side by side: a first kernel
+// makes the state that each piece but a sequence's last adds by itself, and its
+// decay; the scan of a piece then starts from the sum of those before it.
 struct ScanParams {
   SsmParams s;
+  int seg_chunks;      // chunks of a piece; 0: sequences are not divided
+  int max_full;        // grid rows for whole pieces; the last piece of every sequence follows
+  float* seg_state;    // [2 max_full][H][P][N]: pieces' states, then carried states of
+                       // divided sequences (read in place of a state updated in place)
+  float* seg_decay;    // [max_full][H]: log2 of the pieces' decays
 };
+
+struct ScanItem {
+  int seq;             // -1: nothing to do
+  int c0, chunks;      // the piece's chunks within the sequence
+  int first_row;       // row of the sequence's first whole piece in seg_state
+  int piece, pieces;
+  int t_begin, len;    // of the sequence (tokens are below 2^31)
+};
+
+// The piece of grid row `item`.  Whole pieces come first, so that the long work
+// starts first: row r is the r-th whole piece over all sequences, found by a
+// running sum, 32 sequences at a time, by one warp.
+__device__ inline void scan_item(const ScanParams& sp, int item, ScanItem* out) {
+  const SsmParams& p = sp.s;
+  const int lane = threadIdx.x & 31;
+  const int want_seq = item - sp.max_full;   // >= 0: the last piece of that sequence
+  int before = 0, seq = -1, first_row = 0, begin = 0, len = -1, full = 0;
+#pragma unroll 1
+  for (int base = sp.seg_chunks > 0 ? 0 : want_seq; base < p.seqs; base += 32) {
+    const int i = base + lane;
+    begin = 0;
+    len = -1;
+    if (i < p.seqs) {
+      const long long s = index_at(p.cu, p.cu_is64, i), e = index_at(p.cu, p.cu_is64, i + 1);
+      if (s >= 0 && e >= s && e <= p.tokens) {
+        begin = static_cast<int>(s);
+        len = static_cast<int>(e - s);
+      }
+    }
+    full = sp.seg_chunks > 0 && len > 0 ? (len + kScanQ - 1) / kScanQ / sp.seg_chunks : 0;
+    int sum = full;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    const bool here = want_seq >= 0 ? i == want_seq
+                                    : item >= before + sum - full && item < before + sum;
+    const unsigned int hit = __ballot_sync(0xffffffffu, here);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      seq = base + src;
+      first_row = before + __shfl_sync(0xffffffffu, sum - full, src);
+      begin = __shfl_sync(0xffffffffu, begin, src);
+      len = __shfl_sync(0xffffffffu, len, src);
+      full = __shfl_sync(0xffffffffu, full, src);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane != 0) return;
+  ScanItem it;
+  it.seq = seq;
+  it.t_begin = begin;
+  it.len = len;
+  it.first_row = first_row;
+  if (seq >= 0 && len < 0) {
+    atomicOr(p.status, kMixerBadSeqlens);
+    it.seq = -1;
+  }
+  const int nch = (len + kScanQ - 1) / kScanQ;
+  const int rest = nch - full * sp.seg_chunks;
+  it.pieces = full + (rest > 0 || nch == 0 ? 1 : 0);
+  it.piece = want_seq >= 0 ? full : item - first_row;
+  it.chunks = want_seq >= 0 ? rest : sp.seg_chunks;
+  if (want_seq >= 0 && rest == 0 && nch > 0) it.seq = -1;
+  it.c0 = it.piece * sp.seg_chunks;
+  *out = it;
+}
+
+// Waits are warp-uniform and bounded: so many tries, each of which may sleep a
+// microsecond, some tens of milliseconds at least and about a second at most.
+// The first to run out raises the abort flag, which ends every role's loop.
+// (A count takes a fraction of the code of a clock, and the roles' loops have to
+// fit the instruction cache together.)
+constexpr int kScanWaitTries = 1 << 20;
+__device__ __forceinline__ bool scan_try_wait(uint32_t addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+struct ScanSync {
+  uint32_t bars;              // shared-memory address
+  volatile int* abort_flag;   // a status code once a wait ran out
+  __device__ __forceinline__ bool wait(int bar, int phase, int code) const {
+    const uint32_t addr = bars + 8 * bar;
+    int left = kScanWaitTries;
+    while (!__all_sync(0xffffffffu, scan_try_wait(addr, phase & 1))) {
+      if (*abort_flag != 0) return false;
+      if (--left == 0) *abort_flag = code;
+    }
+    return true;
+  }
+  __device__ __forceinline__ void arrive(int bar) const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0)
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bars + 8 * bar) : "memory");
+  }
+};
+
+// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|), in a few units of 2^-24:
+// the exponent's product is carried in two parts, and with z = e / (2 + e),
+// log1p(e) = 2 atanh(z) = 2 (z + z^3 / 3 + z^5 / 5 + ...), z <= 1/3, where the
+// terms from z^15 on are below 2^-26 of the sum.
+__device__ __forceinline__ float scan_step_size(float v) {
+  const float a = fmaxf(-fabsf(v), -150.0f);   // e underflows below; and -inf is a value
+  const float hi = a * 1.4426950408889634f;
+  const float lo = fmaf(a, 1.4426950408889634f, -hi) + a * 1.925963033500e-8f;
+  float e = scan_exp2(hi);
+  e = fmaf(e, lo * 0.6931471805599453f, e);
+  const float z = __fdividef(e, 2.0f + e);
+  const float q = z * z;
+  float s = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
+  s = fmaf(s, q, 1.0f / 9.0f);
+  s = fmaf(s, q, 1.0f / 7.0f);
+  s = fmaf(s, q, 1.0f / 5.0f);
+  s = fmaf(s, q, 1.0f / 3.0f);
+  s = fmaf(s * q, z, z);
+  return v != v ? v : fmaxf(v, 0.0f) + (s + s);
+}
+
+// Accurate to 2^-22 absolutely, which is what a weight's exponent needs.
+__device__ __forceinline__ float scan_log2(float v) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The gates of chunks by one warp, lane owning one token of each block of 32: the
+// steps, the log2 decays after a token to the chunk's end (sfx), after each
+// block (ref), and of the whole chunk.  A chunk's dt are loaded while the one
+// before it (of this warp) is worked on.
+struct ScanGates {
+  const __nv_bfloat16* dt;    // of the piece's first token and this head
+  long long stride;
+  float a2, bias;             // log2 decay per step, and dt_bias
+  int len;                    // tokens of the piece
+  __nv_bfloat16 raw[4];
+  float step[4], sfx[4], ref[4], total;
+  __device__ __forceinline__ void fetch(int c) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int t = c * kScanQ + 32 * b + static_cast<int>(threadIdx.x & 31);
+      raw[b] = __float2bfloat16_rn(0.0f);
+      if (c >= 0 && t < len) raw[b] = dt[t * stride];
+    }
+  }
+  __device__ __forceinline__ void start(const SsmParams& p, long long t_begin, int tokens, int head,
+                                        int c) {
+    dt = p.dt + t_begin * p.dt_stride + head;
+    stride = p.dt_stride;
+    a2 = -expf(p.A_log[head]) * 1.4426950408889634f;
+    bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
+    len = tokens;
+    fetch(c);
+  }
+  __device__ __forceinline__ void make(int c, int next) {
+    const int lane = threadIdx.x & 31;
+    float v[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      step[b] = scan_step_size(to_float(raw[b]) + bias);
+      if (c * kScanQ + 32 * b + lane >= len) step[b] = 0.0f;
+      v[b] = a2 * step[b];
+    }
+    fetch(next);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)   // sums over this lane and those after it
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const float u = __shfl_down_sync(0xffffffffu, v[b], o);
+        if (lane + o < 32) v[b] += u;
+      }
+    total = 0.0f;
+#pragma unroll
+    for (int b = 3; b >= 0; --b) {
+      const float after = __shfl_down_sync(0xffffffffu, v[b], 1);
+      ref[b] = total;
+      sfx[b] = total + (lane == 31 ? 0.0f : after);
+      total += __shfl_sync(0xffffffffu, v[b], 0);
+    }
+  }
+};
+
+// Row `row` of w X, split exactly into three bf16 parts.
+__device__ __forceinline__ void scan_split_row(uint32_t (&part)[3][32], const uint8_t* x, int row,
+                                               float w) {
+  const uint64_t w2 = pair(w, w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint4 u = *reinterpret_cast<const uint4*>(x + sw128_off(row, j));
+    const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint64_t v = mul2(unpack_pair(in[i]), w2);
+      part[0][4 * j + i] = split_pair(v);
+      part[1][4 * j + i] = split_pair(v);
+      part[2][4 * j + i] = pack_pair(v);
+    }
+  }
+}
+
+__device__ __forceinline__ void scan_store_row(uint8_t* xw, const uint32_t (&part)[3][32], int row) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      *reinterpret_cast<uint4*>(xw + k * kScanTile + sw128_off(row, j)) =
+          make_uint4(part[k][4 * j], part[k][4 * j + 1], part[k][4 * j + 2], part[k][4 * j + 3]);
+}
+
+// A weight below this exponent, or a decay, is zero in fp32 whatever the rest.
+constexpr float kScanGone = -300.0f;
+
+// ------------------------------------------------ the states of pieces
+// One CTA per whole piece that is not its sequence's last, and 64 columns of a
+// head: the state it adds, sum over its tokens of e^{L_end - L_s} step_s B_s x_s^T,
+// in one accumulator.  Chunks run from the last to the first, so that weights
+// only need the decays already seen, and end where those leave nothing.
+constexpr int kStateThreads = 384;
+constexpr uint32_t kSsB = 0, kSsX = 2 * kScanTile, kSsStage = 3 * kScanTile;
+constexpr uint32_t kSsXw = 2 * kSsStage;                       // two sets of three tiles
+constexpr uint32_t kSsGate = kSsXw + 6 * kScanTile;            // per stage: exponents [128]
+constexpr uint32_t kSsMisc = kSsGate + 2 * kScanQ * 4;
+constexpr uint32_t kSsItem = kSsMisc + 208;
+constexpr uint32_t kStateSmem = kSsMisc + 256;
+
+enum StateBar {
+  kAFull = 0, kAEmpty = 2, kAGateFull = 4, kAGateEmpty = 6, kAXwFull = 8, kAXwEmpty = 10, kADone = 12,
+  kACount
+};
+
+template <int N>
+__global__ void __launch_bounds__(kStateThreads, 1)
+gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
+                           const __grid_constant__ CUtensorMap tm_b, const ScanParams sp) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const SsmParams& p = sp.s;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int quad = warp & 3, row = quad * 32 + lane;
+  const int units = p.head_dim / kScanCols;
+  const int head = blockIdx.x / units, col0 = blockIdx.x % units * kScanCols;
+  const int group = head / (p.heads / p.groups);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSsMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kSsMisc + 8 * kACount);
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + kSsMisc + 8 * kACount + 4);
+  // log2 decay of the chunks done before a stage's chunk, and including it
+  float* later = reinterpret_cast<float*>(smem + kSsMisc + 8 * kACount + 8);   // [2][2]
+  static_assert(8 * kACount + 24 <= 208 && sizeof(ScanItem) <= 48, "they fit");
+  if (warp == 0) {
+    tmem_alloc(tmem_ptr, 256);
+    tmem_relinquish();
+  }
+  if (warp == 1 && lane == 0) {
+    *abort_flag = 0;
+#pragma unroll 1
+    for (int i = 0; i < kACount; ++i)
+      mbar_init(bars + i, i == kAGateEmpty || i == kAGateEmpty + 1 ? 6   // copies, products, 4 warps
+                          : i == kAXwFull || i == kAXwFull + 1     ? 4
+                                                                   : 1);
+    fence_mbarrier_init();
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_b);
+  }
+  if (warp == 2) scan_item(sp, blockIdx.y, reinterpret_cast<ScanItem*>(smem + kSsItem));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const ScanItem& it = *reinterpret_cast<const ScanItem*>(smem + kSsItem);
+  const int nch = warp_uniform(it.seq < 0 || it.piece == it.pieces - 1 ? 0 : it.chunks);
+  const long long hbase = (static_cast<long long>(head) * p.head_dim + col0) * N;
+  const long long per_slot = static_cast<long long>(p.heads) * p.head_dim * N;
+  const uint32_t tmem = static_cast<uint32_t>(warp_uniform(static_cast<int>(*tmem_ptr)));
+  const int t_last = warp_uniform(it.t_begin + (it.c0 + nch - 1) * kScanQ);
+  const ScanSync sync{smem_u32(bars), abort_flag};
+  // Chunk i of the order, from the end: false once the decays leave nothing of it.
+  auto more = [&](int i) { return later[2 * (i & 1)] > kScanGone; };
+
+  if (nch == 0) {
+    // no such piece, or a sequence's last
+  } else if (warp == 0) {
+    int issued = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < nch; ++i) {
+      const int st = i & 1;
+      if (!(ok = sync.wait(kAGateFull + st, i >> 1, kStatusMmaTimeout))) break;
+      const bool go = more(i);
+      sync.arrive(kAGateEmpty + st);
+      if (!go) break;
+      if (i >= 2 && !(ok = sync.wait(kAEmpty + st, (i >> 1) - 1, kStatusMmaTimeout))) break;
+      if (elect_one()) {
+        uint8_t* stage = smem + st * kSsStage;
+        uint64_t* bar = bars + kAFull + st;
+        const int t0 = t_last - i * kScanQ;
+        mbar_arrive_expect_tx(bar, (1 + N / 64) * kScanTile);
+        tma_load_3d(stage + kSsX, &tm_x, bar, col0, head, t0);
+#pragma unroll
+        for (int b = 0; b < N / 64; ++b)
+          tma_load_3d(stage + kSsB + b * kScanTile, &tm_b, bar, 64 * b, group, t0);
+      }
+      __syncwarp();
+      issued = i + 1;
+    }
+    if (!ok)   // aborted: the copies in flight land first
+      for (int i = max(issued - 2, 0); i < issued; ++i) mbar_wait(bars + kAFull + (i & 1), (i >> 1) & 1);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = idesc_bf16_f32(128, 192, 1, 1);
+    const uint32_t base = smem_u32(smem);
+#pragma unroll 1
+    for (int i = 0; i < nch; ++i) {
+      const int st = i & 1;
+      if (!sync.wait(kAGateFull + st, i >> 1, kStatusMmaTimeout)) break;
+      const bool go = more(i);
+      sync.arrive(kAGateEmpty + st);
+      if (!go) break;
+      if (!sync.wait(kAXwFull + st, i >> 1, kStatusMmaTimeout)) break;   // the copies have landed too
+      tc_fence_after();
+      const uint64_t b_desc = sdesc_sw128(base + st * kSsStage + kSsB, kScanTile, 1024);
+      const uint64_t xw_desc = sdesc_sw128(base + kSsXw + st * 3 * kScanTile, kScanTile, 1024);
+#pragma unroll
+      for (int s = 0; s < kScanQ / 16; ++s)
+        umma_bf16_elect(tmem, sdesc_add(b_desc, s * 2048), sdesc_add(xw_desc, s * 2048), idesc,
+                        i > 0 || s > 0);
+      umma_commit_elect(bars + kAEmpty + st);
+      umma_commit_elect(bars + kAXwEmpty + st);
+    }
+    // the sum is whole, or, after an abort, nothing is in flight any more
+    umma_commit_elect(bars + kADone);
+    mbar_wait(bars + kADone, 0);
+  } else if (warp < 4) {
+    const int last = it.c0 + nch - 1;
+    ScanGates gates;
+    gates.start(p, it.t_begin, it.len, head, warp - 2 < nch ? last - (warp - 2) : -1);
+#pragma unroll 1
+    for (int i = warp - 2; i < nch; i += 2) {
+      const int st = i & 1;
+      gates.make(last - i, i + 2 < nch ? last - i - 2 : -1);
+      float done = 0.0f;   // the other warp's running total
+      bool ended = false;  // at the chunk before: this one only passes that on to its warpgroup
+      if (i > 0) {
+        if (!sync.wait(kAGateFull + (st ^ 1), (i - 1) >> 1, kStatusMmaTimeout)) break;
+        done = later[2 * (st ^ 1) + 1];
+        ended = later[2 * (st ^ 1)] <= kScanGone;
+      }
+      if (i >= 2 && !sync.wait(kAGateEmpty + st, (i >> 1) - 1, kStatusMmaTimeout)) break;
+      float* g = reinterpret_cast<float*>(smem + kSsGate + st * kScanQ * 4);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) g[32 * b + lane] = done + gates.sfx[b] + scan_log2(gates.step[b]);
+      const float total = gates.total;
+      if (lane == 0) {
+        later[2 * st] = done;
+        later[2 * st + 1] = done + total;
+        if (col0 == 0 && !ended && (i == nch - 1 || done <= kScanGone))
+          sp.seg_decay[static_cast<long long>(blockIdx.y) * p.heads + head] = done + total;
+      }
+      sync.arrive(kAGateFull + st);
+      if (done <= kScanGone) break;
+    }
+  } else {
+    // two warpgroups, one chunk each in turn
+    const int wg = (warp - 4) >> 2;
+#pragma unroll 1
+    for (int i = wg; i < nch; i += 2) {
+      const int st = i & 1;
+      if (!sync.wait(kAGateFull + st, i >> 1, kStatusMmaTimeout)) break;
+      const bool go = more(i);
+      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kSsGate + st * kScanQ * 4)[row]);
+      sync.arrive(kAGateEmpty + st);
+      if (!go) break;
+      if (!sync.wait(kAFull + st, i >> 1, kStatusTmaTimeout)) break;
+      uint32_t part[3][32];
+      scan_split_row(part, smem + st * kSsStage + kSsX, row, w);
+      if (i >= 2 && !sync.wait(kAXwEmpty + st, (i >> 1) - 1, kStatusMmaTimeout)) break;
+      scan_store_row(smem + kSsXw + st * 3 * kScanTile, part, row);
+      fence_proxy_async_smem();
+      sync.arrive(kAXwFull + st);
+    }
+    // the result, half of the columns each
+    if (sync.wait(kADone, 0, kStatusMmaTimeout)) {
+      tc_fence_after();
+      float d[3][32];
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        tmem_ld32(tmem + 64 * k + 32 * wg + (static_cast<uint32_t>(quad * 32) << 16), d[k]);
+      tmem_wait_ld();
+      if (row < N) {
+        float* dst = sp.seg_state + blockIdx.y * per_slot + hbase + 32LL * wg * N + row;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          dst[static_cast<long long>(j) * N] = (d[2][j] + d[1][j]) + d[0][j];
+      }
+    }
+    // A state that is updated in place is kept for the first piece, which may
+    // run after the last one has stored its result.
+    const long long slot = slot_of(p.slots, p.slots_is64, it.seq, p.pool, p.status, false);
+    if (it.piece == 0 && p.state == p.new_state && slot >= 0) {
+      float* dst = sp.seg_state + (sp.max_full + it.first_row) * per_slot + hbase;
+      for (int e = threadIdx.x - 128; e < kScanCols * N; e += kStateThreads - 128)
+        dst[e] = p.state[slot * per_slot + hbase + e];
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, static_cast<unsigned int>(*abort_flag));
+  if (warp == 0) tmem_dealloc(tmem, 256);
+}
 
 template <int N>
 __global__ void __launch_bounds__(kScanThreads, 1)
@@ -138,39 +576,20 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                     const __grid_constant__ CUtensorMap tm_c, const ScanParams sp) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const SsmParams& p = sp.s;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int quad = warp & 3, row = quad * 32 + lane;
   const int units = p.head_dim / kScanCols;
   const int head = blockIdx.x / units, col0 = blockIdx.x % units * kScanCols;
   const int group = head / (p.heads / p.groups);
-  const int seq = blockIdx.y;
-  const bool reporter = blockIdx.x == 0 && threadIdx.x == 0;
-
-  const long long t_begin = index_at(p.cu, p.cu_is64, seq);
-  const long long t_end = index_at(p.cu, p.cu_is64, seq + 1);
-  if (t_begin < 0 || t_end < t_begin || t_end > p.tokens) {
-    if (reporter) atomicOr(p.status, kMixerBadSeqlens);
-    return;
-  }
-  const int len = static_cast<int>(t_end - t_begin);
-  const int nch = (len + kScanQ - 1) / kScanQ;
-  const long long slot = slot_of(p.slots, p.slots_is64, seq, p.pool, p.status, reporter);
-  const bool carried = p.state && slot >= 0 && (!p.has_state || p.has_state[seq]);
-  const long long sbase =
-      ((slot < 0 ? 0 : slot) * p.heads + head) * static_cast<long long>(p.head_dim) * N +
-      static_cast<long long>(col0) * N;
-  if (nch == 0) {   // nothing but the state
-    if (slot >= 0)
-      for (int e = threadIdx.x; e < kScanCols * N; e += kScanThreads)
-        p.new_state[sbase + e] = carried ? p.state[sbase + e] : 0.0f;
-    return;
-  }
-
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kScMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kScMisc + 8 * kBCount);
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + kScMisc + 8 * kBCount + 4);
-  float* totals = reinterpret_cast<float*>(smem + kScMisc + 8 * kBCount + 8);   // [2]
-  static_assert(8 * kBCount + 16 <= 256, "barriers and flags fit");
+  // per stage, the decay of each 32 tokens of the chunk
+  float* totals = reinterpret_cast<float*>(smem + kScMisc + 8 * kBCount + 8);   // [2][4]
+  auto chunk_total = [&](int st) {
+    return (totals[4 * st + 3] + totals[4 * st + 2]) + totals[4 * st + 1] + totals[4 * st];
+  };
+  static_assert(8 * kBCount + 40 <= 224 && sizeof(ScanItem) <= 32, "they fit");
 
   if (warp == 0) {
     tmem_alloc(tmem_ptr, 512);
@@ -178,12 +597,14 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   }
   if (warp == 1 && lane == 0) {
     *abort_flag = 0;
+#pragma unroll 1
     for (int i = 0; i < kBCount; ++i) {
       int n = 1;
       if (i == kBEmpty || i == kBEmpty + 1) n = 1 + 4;   // products, output warps
-      else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 12;
+      else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 16;
       else if (i == kBEmptyC0 || i == kBEmptyC0 + 1 || i == kBMFull || i == kBYEmpty ||
-               i == kBXwFull || i == kBHFull)
+               i == kBXwFull || i == kBHFull || i == kBDsEmpty || i == kBGateFull || i == kBGateFull + 1 ||
+               i == kBGateSum)
         n = 4;
       mbar_init(bars + i, n);
     }
@@ -192,27 +613,43 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     prefetch_tmap(&tm_b);
     prefetch_tmap(&tm_c);
   }
+  if (warp == 2) scan_item(sp, blockIdx.y, reinterpret_cast<ScanItem*>(smem + kScItem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_ptr;
+  const ScanItem& it = *reinterpret_cast<const ScanItem*>(smem + kScItem);
+  const int nch = warp_uniform(it.seq < 0 ? 0 : it.chunks);
+  const int t_begin = warp_uniform(it.t_begin + it.c0 * kScanQ);
+  const int len = warp_uniform(min(it.len - it.c0 * kScanQ, nch * kScanQ));
+  const long long hbase = (static_cast<long long>(head) * p.head_dim + col0) * N;
+  const long long per_slot = static_cast<long long>(p.heads) * p.head_dim * N;
+  const uint32_t tmem = static_cast<uint32_t>(warp_uniform(static_cast<int>(*tmem_ptr)));
   const uint32_t tm_lane = static_cast<uint32_t>(quad * 32) << 16;
 
-  // Waits are warp-uniform and bounded; the first to run out raises the abort
-  // flag, which ends every role's loop.
-  auto wait = [&](int bar, int phase, unsigned int code) {
-    const int r = mbar_wait_or_abort(bars + bar, phase & 1, abort_flag);
-    if (r < 0) atomicOr(p.status, code);
-    return __all_sync(0xffffffffu, r == 1);
-  };
-  auto arrive = [&](int bar) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bars + bar);
-  };
+  const ScanSync sync{smem_u32(bars), abort_flag};
+  auto wait = [&](int bar, int phase, int code) { return sync.wait(bar, phase, code); };
+  auto arrive = [&](int bar) { sync.arrive(bar); };
   auto chunk_len = [&](int c) { return min(kScanQ, len - c * kScanQ); };
+  // The sequence's slot, and whether it starts from a carried state.
+  auto find_state = [&](bool& carried) {
+    const long long slot = slot_of(p.slots, p.slots_is64, it.seq, p.pool, p.status,
+                                   blockIdx.x == 0 && (threadIdx.x & 31) == 0);
+    carried = p.state && slot >= 0 && (!p.has_state || p.has_state[it.seq]);
+    return slot;
+  };
   constexpr int kSteps = N / 16;   // k-steps over the state dimension
 
-  if (warp < 4) {
+  if (nch == 0) {
+    if (it.seq >= 0) {   // an empty sequence: nothing but the state
+      bool carried;
+      const long long slot = find_state(carried);
+      if (slot >= 0)
+        for (int e = threadIdx.x; e < kScanCols * N; e += kScanThreads) {
+          const long long at = slot * per_slot + hbase + e;
+          p.new_state[at] = carried ? p.state[at] : 0.0f;
+        }
+    }
+  } else if (warp < 4) {
     scan_set_regs<kScanRegs[0]>();
     if (warp == 0) {
       // ---------------------------------------------- TMA
@@ -220,10 +657,11 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       // pass through it.
       int issued = 0;
       bool ok = true;
+#pragma unroll 1
       for (int c = 0; c < nch; ++c) {
         const int st = c & 1;
         uint8_t* stage = smem + st * kScStage;
-        const int t0 = static_cast<int>(t_begin) + c * kScanQ;
+        const int t0 = t_begin + c * kScanQ;
         if (c >= 2 && !(ok = wait(kBEmpty + st, (c >> 1) - 1, kStatusMmaTimeout))) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(bars + kBFullX + st, kScanTile);
@@ -249,142 +687,125 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         }
     } else if (warp == 1) {
       // ---------------------------------------------- products
+      // Every lane runs the whole sequence and an elected one issues: the warp
+      // never diverges, so descriptors stay in uniform registers.  (Inside a
+      // branch on the elected lane each product took twice as long to issue, and
+      // in a loop over k-steps four times.)
       constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, 0, 0);
       constexpr uint32_t idesc_y = idesc_bf16_f32(128, 64, 0, 1);
       constexpr uint32_t idesc_ds = idesc_bf16_f32(128, 192, 1, 1);
       const uint32_t base = smem_u32(smem);
-      auto issue_s = [&](int c) {
-        const uint32_t st = base + (c & 1) * kScStage;
-        if (elect_one()) {
+      const uint64_t xw_desc = sdesc_sw128(base + kScXw, kScanTile, 1024);
+      const uint64_t h_desc = sdesc_sw128(base + kScH, kScanTile, 1024);
+      bool ok = true;
+#pragma unroll 1
+      for (int c = -1; c < nch; ++c) {
+        if (c >= 0) {
+          const uint32_t st = base + (c & 1) * kScStage;
+          const uint64_t bt_desc = sdesc_sw128(st + kScB, kScanTile, 1024);
+          const uint64_t c_desc = sdesc_sw128(st + kScC, 16, 1024);
+          const uint64_t x_desc = sdesc_sw128(st + kScX, kScanTile, 1024);
+          if (!(ok = wait(kBXwFull, c, kStatusMmaTimeout))) break;
+          if (c > 0 && !(ok = wait(kBDsEmpty, c - 1, kStatusMmaTimeout))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kScanQ / 16; ++s)
+            umma_bf16_elect(tmem + kTmDs, sdesc_add(bt_desc, s * 2048), sdesc_add(xw_desc, s * 2048),
+                            idesc_ds, s > 0);
+          umma_commit_elect(bars + kBDsFull);
+          if (!(ok = wait(kBHFull, c, kStatusMmaTimeout))) break;
+          if (c > 0 && !(ok = wait(kBYEmpty, c - 1, kStatusMmaTimeout))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s)
+            umma_bf16_elect(tmem + kTmYo, sdesc_add(c_desc, (s >> 2) * kScanTile + (s & 3) * 32),
+                            sdesc_add(h_desc, s * 2048), idesc_y, s > 0);
+          umma_commit_elect(bars + kBHEmpty);
+          if (!(ok = wait(kBMFull, c, kStatusMmaTimeout))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kScanQ / 16; ++s)
+            umma_bf16_ts_elect(tmem + kTmYd, tmem + kTmM + s * 8, sdesc_add(x_desc, s * 2048),
+                               idesc_y, s > 0);
+          umma_commit_elect(bars + kBYFull);
+          if (c + 2 < nch) umma_commit_elect(bars + kBEmpty + (c & 1));
+        }
+        if (c + 1 < nch) {   // M of this chunk is made, so S is read
+          const uint32_t st = base + ((c + 1) & 1) * kScStage;
+          const uint64_t c_desc = sdesc_sw128(st + kScC, 16, 1024);
+          const uint64_t b_desc = sdesc_sw128(st + kScB, 16, 1024);
+          if (!(ok = wait(kBFullBC + ((c + 1) & 1), (c + 1) >> 1, kStatusTmaTimeout))) break;
+          tc_fence_after();
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             const uint32_t off = (s >> 2) * kScanTile + (s & 3) * 32;
-            umma_bf16(tmem + kTmS, sdesc_sw128(st + kScC + off, 16, 1024),
-                      sdesc_sw128(st + kScB + off, 16, 1024), idesc_s, s > 0);
+            umma_bf16_elect(tmem + kTmS, sdesc_add(c_desc, off), sdesc_add(b_desc, off), idesc_s, s > 0);
           }
-          umma_commit(bars + kBSFull);
-        }
-        __syncwarp();
-      };
-      bool ok = wait(kBFullBC, 0, kStatusTmaTimeout);
-      if (ok) issue_s(0);
-      for (int c = 0; ok && c < nch; ++c) {
-        const uint32_t st = base + (c & 1) * kScStage;
-        const int ksteps = (chunk_len(c) + 15) / 16;
-        if (!(ok = wait(kBXwFull, c, kStatusMmaTimeout))) break;
-        tc_fence_after();
-        if (elect_one()) {
-          for (int s = 0; s < ksteps; ++s)
-            umma_bf16(tmem + kTmDs, sdesc_sw128(st + kScB + s * 2048, kScanTile, 1024),
-                      sdesc_sw128(base + kScXw + s * 2048, kScanTile, 1024), idesc_ds, s > 0);
-          umma_commit(bars + kBDsFull);
-        }
-        __syncwarp();
-        if (!(ok = wait(kBHFull, c, kStatusMmaTimeout))) break;
-        if (c > 0 && !(ok = wait(kBYEmpty, c - 1, kStatusMmaTimeout))) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s)
-            umma_bf16(tmem + kTmYo,
-                      sdesc_sw128(st + kScC + (s >> 2) * kScanTile + (s & 3) * 32, 16, 1024),
-                      sdesc_sw128(base + kScH + s * 2048, kScanTile, 1024), idesc_y, s > 0);
-          umma_commit(bars + kBHEmpty);
-        }
-        __syncwarp();
-        if (!(ok = wait(kBMFull, c, kStatusMmaTimeout))) break;
-        tc_fence_after();
-        if (elect_one()) {
-          for (int s = 0; s < ksteps; ++s)
-            umma_bf16_ts(tmem + kTmYd, tmem + kTmM + s * 8,
-                         sdesc_sw128(st + kScX + s * 2048, kScanTile, 1024), idesc_y, s > 0);
-          umma_commit(bars + kBYFull);
-          if (c + 2 < nch) umma_commit(bars + kBEmpty + (c & 1));
-        }
-        __syncwarp();
-        if (c + 1 < nch) {   // M of this chunk is made, so S is read
-          if (!(ok = wait(kBFullBC + ((c + 1) & 1), (c + 1) >> 1, kStatusTmaTimeout))) break;
-          issue_s(c + 1);
+          umma_commit_elect(bars + kBSFull);
         }
       }
       if (!ok) {   // aborted: the products in flight finish first
-        if (elect_one()) umma_commit(bars + kBDrain);
-        __syncwarp();
+        umma_commit_elect(bars + kBDrain);
         mbar_wait(bars + kBDrain, 0);
-      }
-    } else {
-      // ---------------------------------------------- gates
-      // Two warps take turns; a chunk's dt are on their way while the chunk
-      // before it (of this warp) is worked on.
-      const float a2 = -expf(p.A_log[head]) * 1.4426950408889634f;
-      const float bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
-      const __nv_bfloat16* dt = p.dt + t_begin * p.dt_stride + head;
-      __nv_bfloat16 raw[4];
-      auto load_dt = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = c * kScanQ + 4 * lane + i;
-          raw[i] = __float2bfloat16_rn(0.0f);
-          if (t < len) raw[i] = dt[t * p.dt_stride];
-        }
-      };
-      load_dt(warp - 2);
-      for (int c = warp - 2; c < nch; c += 2) {
-        const int st = c & 1, n = chunk_len(c);
-        float step[4], la[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          step[i] = 4 * lane + i < n ? ssm_step_size(to_float(raw[i]) + bias) : 0.0f;
-          la[i] = a2 * step[i];
-        }
-        load_dt(c + 2);
-        float sfx[4];
-        sfx[3] = 0.0f;
-        sfx[2] = la[3];
-        sfx[1] = sfx[2] + la[2];
-        sfx[0] = sfx[1] + la[1];
-        float v = sfx[0] + la[0];   // sums over this lane and those after it
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float u = __shfl_down_sync(0xffffffffu, v, o);
-          if (lane + o < 32) v += u;
-        }
-        float after = __shfl_down_sync(0xffffffffu, v, 1);
-        if (lane == 31) after = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sfx[i] += after;
-        // the last token of this lane's 32
-        const float ref = __shfl_sync(0xffffffffu, sfx[3], lane | 7);
-        if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) break;
-        float* g = reinterpret_cast<float*>(smem + kScGate + st * kScGateStage);
-        reinterpret_cast<float4*>(g + kScanQ)[lane] = make_float4(sfx[0], sfx[1], sfx[2], sfx[3]);
-        // log2 of a zero step is -inf: a padded token has no weight anywhere
-        reinterpret_cast<float4*>(g)[lane] =
-            make_float4(sfx[0] + log2f(step[0]), sfx[1] + log2f(step[1]), sfx[2] + log2f(step[2]),
-                        sfx[3] + log2f(step[3]));
-        if (lane < 24)
-          reinterpret_cast<float4*>(g + 2 * kScanQ)[lane] =
-              make_float4(step[0] * scan_exp2(sfx[0] - ref), step[1] * scan_exp2(sfx[1] - ref),
-                          step[2] * scan_exp2(sfx[2] - ref), step[3] * scan_exp2(sfx[3] - ref));
-        if (lane == 0) totals[st] = v;
-        arrive(kBGateFull + st);
       }
     }
   } else if (warp < 8) {
     // ------------------------------------------------ S -> M
     scan_set_regs<kScanRegs[1]>();
+    // The gates, thread = token: a suffix sum over the chunk in the warp, and over
+    // the four warps through shared memory.  Those of the next chunk are made
+    // while this one's S is.
+    const float a2 = -expf(p.A_log[head]) * 1.4426950408889634f;
+    const float bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
+    const __nv_bfloat16* dt = p.dt + t_begin * p.dt_stride + head;
+    __nv_bfloat16 raw = __float2bfloat16_rn(0.0f);
+    if (row < len) raw = dt[row * p.dt_stride];
+    auto make_gates = [&](int c) {
+      const int st = c & 1, t = c * kScanQ + row;
+      float step = scan_step_size(to_float(raw) + bias);
+      if (t >= len) step = 0.0f;
+      if (t + kScanQ < len) raw = dt[(t + kScanQ) * p.dt_stride];
+      float v = a2 * step;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {   // sums over this lane and those after it
+        const float u = __shfl_down_sync(0xffffffffu, v, o);
+        if (lane + o < 32) v += u;
+      }
+      float sfx = __shfl_down_sync(0xffffffffu, v, 1);
+      if (lane == 31) sfx = 0.0f;
+      if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) return false;
+      float* g = reinterpret_cast<float*>(smem + kScGate + st * kScGateStage);
+      float* sums = totals + 4 * st;
+      if (lane == 0) sums[quad] = v;
+      arrive(kBGateSum);
+      if (!wait(kBGateSum, c, kStatusMmaTimeout)) return false;
+      const float before_last = sfx;
+      float ref = 0.0f;                    // decays of the blocks after this one
+      for (int b = 3; b > quad; --b) ref += sums[b];
+      sfx += ref;
+      // log2 of a zero step is -inf: a padded token has no weight anywhere
+      g[row] = sfx + scan_log2(step);
+      g[kScanQ + row] = sfx;
+      if (quad < 3) g[2 * kScanQ + row] = step * scan_exp2(before_last);
+      arrive(kBGateFull + st);
+      return true;
+    };
+    bool ok = make_gates(0);
     {   // blocks above the diagonal stay zero
       const uint32_t z[16] = {};
       for (int b = quad + 1; b < 4; ++b) tmem_st16(tmem + kTmM + 16 * b + tm_lane, z);
       tmem_wait_st();
     }
-    for (int c = 0; c < nch; ++c) {
+#pragma unroll 1
+    for (int c = 0; ok && c < nch; ++c) {
       const int st = c & 1;
+      if (c + 1 < nch && !make_gates(c + 1)) break;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
       const float* g = reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage);
       const float mine = g[kScanQ + row];
       if (!wait(kBSFull, c, kStatusMmaTimeout)) break;   // also: the last M is read
       tc_fence_after();
+#pragma unroll 1
       for (int b = 0; b < quad; ++b) {
         float s[32];
         tmem_ld32(tmem + kTmS + 32 * b + tm_lane, s);
@@ -426,85 +847,41 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       arrive(kBGateEmpty + st);
     }
   } else if (warp < 12) {
-    // ------------------------------------------------ w X and the state
+    // ------------------------------------------------ the state
     scan_set_regs<kScanRegs[2]>();
     const bool state_row = row < N;
     uint64_t h[kScanCols / 2];
 #pragma unroll
-    for (int j = 0; j < kScanCols / 2; ++j) {
-      const float* src = p.state + sbase + static_cast<long long>(2 * j) * N + row;
-      const bool read = carried && state_row;
-      h[j] = pair(read ? src[0] : 0.0f, read ? src[N] : 0.0f);
-    }
-    auto add_ds = [&](float decay) {
-      const uint64_t d2 = pair(decay, decay);
+    for (int j = 0; j < kScanCols / 2; ++j) h[j] = 0ull;
+    auto add_state = [&](const float* src, float log_decay) {
+      const float f = scan_exp2(log_decay);
+      const uint64_t f2 = pair(f, f);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        float d[3][32];
-#pragma unroll
-        for (int k = 0; k < 3; ++k) tmem_ld32(tmem + kTmDs + 64 * k + 32 * b + tm_lane, d[k]);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {   // the small parts first
-          const uint64_t t = add2(add2(pair(d[2][2 * j], d[2][2 * j + 1]),
-                                       pair(d[1][2 * j], d[1][2 * j + 1])),
-                                  pair(d[0][2 * j], d[0][2 * j + 1]));
-          h[16 * b + j] = fma2(h[16 * b + j], d2, t);
-        }
+      for (int j = 0; j < kScanCols / 2; ++j) {
+        const float* s = src + 2 * j * N + row;
+        h[j] = fma2(pair(__ldg(s), __ldg(s + N)), f2, h[j]);
       }
     };
+    bool carried;
+    const long long slot = find_state(carried);
+    if (state_row) {   // the start: what the pieces before this one leave, and the carried state
+      float log_decay = 0.0f;
+#pragma unroll 1
+      for (int r = it.piece - 1; r >= (carried ? -1 : 0) && log_decay > kScanGone; --r) {
+        const float* src = sp.seg_state + (it.first_row + r) * per_slot + hbase;
+        if (r < 0)
+          src = it.pieces > 1 && p.state == p.new_state
+                    ? sp.seg_state + (sp.max_full + it.first_row) * per_slot + hbase
+                    : p.state + slot * per_slot + hbase;
+        add_state(src, log_decay);
+        if (r >= 0)
+          log_decay += sp.seg_decay[static_cast<long long>(it.first_row + r) * p.heads + head];
+      }
+    }
     bool ok = true;
-    float decay = 1.0f;
-    for (int c = 0; c < nch; ++c) {
-      const int st = c & 1, n = chunk_len(c);
-      uint8_t* stage = smem + st * kScStage;
-      if (!(ok = wait(kBGateFull + st, c >> 1, kStatusMmaTimeout))) break;
-      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[row]);
-      const float next_decay = scan_exp2(totals[st]);
-      arrive(kBGateEmpty + st);
-      if (c > 0) {
-        if (!(ok = wait(kBDsFull, c - 1, kStatusMmaTimeout))) break;
-        tc_fence_after();
-        add_ds(decay);
-        tc_fence_before();
-      }
-      decay = next_decay;
-      if (!(ok = wait(kBFullX + st, c >> 1, kStatusTmaTimeout))) break;
-      if (n < kScanQ) {   // a last, short chunk: what lies past it must not count
-        if (!(ok = wait(kBFullBC + st, c >> 1, kStatusTmaTimeout))) break;
-        if (row >= n) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t off = sw128_off(row, j);
-            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(stage + kScX + off) = z;
-#pragma unroll
-            for (int b = 0; b < N / 64; ++b)
-              *reinterpret_cast<uint4*>(stage + kScB + b * kScanTile + off) = z;
-          }
-        }
-      }
-      const uint64_t w2 = pair(w, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t off = sw128_off(row, j);
-        const uint4 u = *reinterpret_cast<const uint4*>(stage + kScX + off);
-        const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-        uint32_t part[3][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint64_t v = mul2(unpack_pair(in[i]), w2);
-          part[0][i] = split_pair(v);
-          part[1][i] = split_pair(v);
-          part[2][i] = pack_pair(v);
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          *reinterpret_cast<uint4*>(smem + kScXw + k * kScanTile + off) =
-              make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
-      }
-      fence_proxy_async_smem();
-      arrive(kBXwFull);
+#pragma unroll 1
+    for (int c = 0;; ++c) {
+      const int st = c & 1;
       if (c > 0 && !(ok = wait(kBHEmpty, c - 1, kStatusMmaTimeout))) break;
       if (state_row) {
 #pragma unroll
@@ -515,32 +892,83 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       }
       fence_proxy_async_smem();
       arrive(kBHFull);
-    }
-    if (ok && wait(kBDsFull, nch - 1, kStatusMmaTimeout)) {
+      if (!(ok = wait(kBGateFull + st, c >> 1, kStatusMmaTimeout))) break;
+      const float decay = scan_exp2(chunk_total(st));
+      const uint64_t d2 = pair(decay, decay);
+      arrive(kBGateEmpty + st);
+      if (!(ok = wait(kBDsFull, c, kStatusMmaTimeout))) break;
       tc_fence_after();
-      add_ds(decay);
-      tc_fence_before();
-      if (slot >= 0 && state_row) {
 #pragma unroll
-        for (int j = 0; j < kScanCols / 2; ++j) {
-          float* dst = p.new_state + sbase + static_cast<long long>(2 * j) * N + row;
-          const float2 f = unpair(h[j]);
-          dst[0] = f.x;
-          dst[N] = f.y;
+      for (int b = 0; b < 4; ++b) {
+        uint32_t d[3][16];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) tmem_ld16(tmem + kTmDs + 64 * k + 16 * b + tm_lane, d[k]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {   // the small parts first
+          const uint64_t t = add2(add2(pair_bits(d[2][2 * j], d[2][2 * j + 1]),
+                                       pair_bits(d[1][2 * j], d[1][2 * j + 1])),
+                                  pair_bits(d[0][2 * j], d[0][2 * j + 1]));
+          h[8 * b + j] = fma2(h[8 * b + j], d2, t);
         }
       }
+      tc_fence_before();
+      arrive(kBDsEmpty);
+      if (c == nch - 1) break;
+    }
+    if (ok && slot >= 0 && it.piece == it.pieces - 1 && state_row) {
+      float* dst = p.new_state + slot * per_slot + hbase + row;
+#pragma unroll
+      for (int j = 0; j < kScanCols / 2; ++j) {
+        const float2 f = unpair(h[j]);
+        dst[2 * j * N] = f.x;
+        dst[(2 * j + 1) * N] = f.y;
+      }
+    }
+  } else if (warp >= 16) {
+    // ------------------------------------------------ w X
+    scan_set_regs<kScanRegs[4]>();
+#pragma unroll 1
+    for (int c = 0; c < nch; ++c) {
+      const int st = c & 1, n = chunk_len(c);
+      uint8_t* stage = smem + st * kScStage;
+      if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
+      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[row]);
+      arrive(kBGateEmpty + st);
+      if (!wait(kBFullX + st, c >> 1, kStatusTmaTimeout)) break;
+      if (n < kScanQ) {   // a last, short chunk: what lies past it must not count
+        if (!wait(kBFullBC + st, c >> 1, kStatusTmaTimeout)) break;
+        if (row >= n) {
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t off = sw128_off(row, j);
+            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(stage + kScX + off) = z;
+#pragma unroll
+            for (int b = 0; b < N / 64; ++b)
+              *reinterpret_cast<uint4*>(stage + kScB + b * kScanTile + off) = z;
+          }
+        }
+      }
+      uint32_t part[3][32];
+      scan_split_row(part, stage + kScX, row, w);
+      if (c > 0 && !wait(kBDsFull, c - 1, kStatusMmaTimeout)) break;   // the last w X is read
+      scan_store_row(smem + kScXw, part, row);
+      fence_proxy_async_smem();
+      arrive(kBXwFull);
     }
   } else {
     // ------------------------------------------------ outputs
     scan_set_regs<kScanRegs[3]>();
     const float D = p.D ? p.D[head] : 0.0f;
     const uint64_t D2 = pair(D, D);
+#pragma unroll 1
     for (int c = 0; c < nch; ++c) {
       const int st = c & 1, n = chunk_len(c);
       uint8_t* stage = smem + st * kScStage;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
       const float e = scan_exp2(
-          totals[st] - reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row]);
+          chunk_total(st) - reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row]);
       arrive(kBGateEmpty + st);
       if (!wait(kBFullX + st, c >> 1, kStatusTmaTimeout)) break;
       uint4 x[8];   // kept here so that the stage can be refilled early
@@ -553,35 +981,33 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       // the row's results go to C's first half in shared memory (no product
       // reads it any more), from where the warp writes whole rows
       const uint64_t e2 = pair(e, e);
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        float yd[32], yo[32];
-        tmem_ld32(tmem + kTmYd + 32 * b + tm_lane, yd);
-        tmem_ld32(tmem + kTmYo + 32 * b + tm_lane, yo);
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {   // 16 columns at a time
+        uint32_t yd[16], yo[16];
+        tmem_ld16(tmem + kTmYd + 16 * b + tm_lane, yd);
+        tmem_ld16(tmem + kTmYo + 16 * b + tm_lane, yo);
         tmem_wait_ld();
-        if (b == 1) {
-          tc_fence_before();
-          arrive(kBYEmpty);
-        }
+        const uint32_t in[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+        uint32_t out[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t in[4] = {x[4 * b + j].x, x[4 * b + j].y, x[4 * b + j].z, x[4 * b + j].w};
-          uint32_t out[4];
+        for (int i = 0; i < 8; ++i)
+          out[i] = pack_pair(fma2(D2, unpack_pair(in[i]),
+                                  fma2(e2, pair_bits(yo[2 * i], yo[2 * i + 1]),
+                                       pair_bits(yd[2 * i], yd[2 * i + 1]))));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = 8 * j + 2 * i;
-            out[i] = pack_pair(fma2(D2, unpack_pair(in[i]),
-                                    fma2(e2, pair(yo[k], yo[k + 1]), pair(yd[k], yd[k + 1]))));
-          }
-          *reinterpret_cast<uint4*>(stage + kScC + sw128_off(row, 4 * b + j)) =
-              make_uint4(out[0], out[1], out[2], out[3]);
-        }
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<uint4*>(stage + kScC + sw128_off(row, 2 * b + j)) =
+              make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
+#pragma unroll
+        for (int j = 0; j < 6; ++j) x[j] = x[j + 2];
       }
+      tc_fence_before();
+      arrive(kBYEmpty);
       __syncwarp();
       __nv_bfloat16* out = p.out +
-          ((t_begin + static_cast<long long>(c) * kScanQ) * p.heads + head) * p.head_dim + col0;
+          ((static_cast<long long>(t_begin) + c * kScanQ) * p.heads + head) * p.head_dim + col0;
       const long long ld = static_cast<long long>(p.heads) * p.head_dim;
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < 8; ++i) {
         const int r = quad * 32 + 4 * i + (lane >> 3);
         const uint4 u = *reinterpret_cast<const uint4*>(stage + kScC + sw128_off(r, lane & 7));
@@ -594,6 +1020,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, static_cast<unsigned int>(*abort_flag));
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 

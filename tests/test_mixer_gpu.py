@@ -234,6 +234,45 @@ def test_scan_long_sequence():
     run_scan([3000, 10, 1111], 2, 128, 2, 64, seed=6)
 
 
+@pytest.mark.parametrize("strong", [False, True])
+def test_scan_divided_sequences_in_place(strong):
+    """Few heads and long sequences run in pieces; slots in a pool, updated in place,
+    with decays that end within a piece and that reach over several."""
+    lens = [1300, 3, 0, 2048, 512, 700]
+    slots = torch.tensor([6, 0, 3, 1, -1, 4], dtype=torch.int32).cuda()
+    has = torch.tensor([True, True, True, True, True, False]).cuda()
+    assert M.ssm_prefill_workspace_bytes(len(lens), sum(lens), 3, 64, 128) > 0
+    ins, st, cu, out, ns = run_scan(lens, 3, 64, 1, 128, slots=slots, has=has, pool=8,
+                                    strong=strong, seed=21)
+    again = torch.empty_like(out)
+    M.gdn_ssm_prefill(*ins, st, cu, again, st, state_indices=slots, has_state=has)
+    assert torch.equal(again, out) and torch.equal(st, ns)
+
+
+def test_scan_weak_decay_over_pieces():
+    """A head that hardly forgets: every piece counts to the end."""
+    ins = list(scan_inputs(2000, 2, 128, 1, 64, seed=31))
+    ins[2] = torch.full((2,), -9.0).cuda()               # log decay of about 1e-4 a token
+    cu, st = offsets([2000]), rand(1, 2, 128, 64, seed=32)
+    out, ns = torch.empty(2000, 2, 128, dtype=BF).cuda(), torch.empty_like(st)
+    M.gdn_ssm_prefill(*ins, st, cu, out, ns)
+    want, wp, mag, pmag = O.scan(*ins, st, cu, ns)
+    check(out, want, mag, PROMPT_REL, "output")
+    check(ns, wp, pmag, PROMPT_STATE_REL, "state")
+    # the same without a workspace's pieces
+    lib = _lib.load()
+    x, dt, A_log, B, C, D, bias = ins
+    one, ns1 = torch.empty_like(out), torch.empty_like(ns)
+    rc = lib.gdn_b200_ssm_prefill(
+        x.data_ptr(), x.stride(0), dt.data_ptr(), dt.stride(0), A_log.data_ptr(), B.data_ptr(),
+        B.stride(0), C.data_ptr(), C.stride(0), D.data_ptr(), bias.data_ptr(), st.data_ptr(),
+        cu.data_ptr(), 0, 0, 0, 0, one.data_ptr(), ns1.data_ptr(), 1, 2000, 1, 2, 1, 128, 64, 0, 0,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    check(one, want, mag, PROMPT_REL, "output")
+    check(ns1, wp, pmag, PROMPT_STATE_REL, "state")
+
+
 def test_scan_without_skip_and_bias():
     x, dt, A_log, B, C, _, _ = scan_inputs(150, 4, 64, 1, 64)
     dt = dt - 3
