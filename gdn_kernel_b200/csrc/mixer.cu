@@ -199,33 +199,44 @@ int scan_setup() {
   return GDN_B200_OK;
 }
 
-// How a call's sequences are divided.  A CTA runs 64 columns of a head; with
-// fewer (sequence, CTA) pairs than keep the SMs busy, long sequences run in
-// pieces.  Pieces of 1 / (2 SMs) of all chunks leave two or three CTAs to each
-// SM, enough to even out; below kScanMinPiece chunks a piece costs more in
-// starting up than it saves.
-constexpr int kScanPiecesPerSm = 1;
-constexpr int kScanSms = 148, kScanMinPiece = 4, kScanMaxDivided = 1024;
+// How a call's sequences are divided.  A CTA runs 64 columns of a head, one per
+// SM; its start costs about as much as two or three chunks.
+//  * One sequence: as many equal pieces as fill the SMs once.  8,192 tokens of 64
+//    heads run in two pieces; five pieces, with their start-ups, took longer.
+//  * Several: a piece is an SM's share of all chunks, so that a sequence that is
+//    longer than that cannot hold up the rest, and most are not divided.
+// The parts of pieces whose states the first kernel makes fill the SMs likewise.
+constexpr int kScanSms = 148, kScanMinPiece = 4, kScanMaxDivided = 1024, kScanMaxParts = 4;
 
 struct ScanPlan {
   int seg_chunks;        // 0: not divided
+  int parts;
   long long max_full;    // bound on the whole pieces
   size_t state_bytes, bytes;
 };
 
 ScanPlan scan_plan(long long seqs, long long tokens, int heads, int head_dim, int state_dim) {
   ScanPlan plan{};
-  const long long chunks = tokens / kScanQ + seqs;   // no fewer than there are
+  plan.parts = 1;
+  const long long chunks = (tokens + kScanQ - 1) / kScanQ;
   const long long units = static_cast<long long>(heads) * (head_dim / kScanCols);
   if (seqs > kScanMaxDivided || seqs * units >= 8 * kScanSms) return plan;
-  const long long piece =
-      std::max<long long>(kScanMinPiece, (tokens / kScanQ * units + kScanPiecesPerSm * kScanSms - 1) / (kScanPiecesPerSm * kScanSms));
-  if (tokens / kScanQ < piece) return plan;
+  long long piece = (chunks * units + kScanSms - 1) / kScanSms;
+  if (seqs == 1) {
+    const long long pieces = std::max<long long>(1, kScanSms / units);
+    piece = (chunks + pieces - 1) / pieces;
+  }
+  piece = std::max<long long>(piece, kScanMinPiece);
+  if (chunks <= piece) return plan;
+  const long long whole = seqs == 1 ? (chunks - 1) / piece : 1;   // pieces whose states are needed
+  plan.parts = static_cast<int>(
+      std::min<long long>(kScanMaxParts, std::max<long long>(1, kScanSms / (units * whole))));
+  piece = (piece + plan.parts - 1) / plan.parts * plan.parts;
   plan.seg_chunks = static_cast<int>(piece);
-  plan.max_full = chunks / piece;
+  plan.max_full = (chunks + seqs) / piece;
   const size_t row = static_cast<size_t>(heads) * head_dim * state_dim * 4;
-  plan.state_bytes = 2 * plan.max_full * row;
-  plan.bytes = plan.state_bytes + plan.max_full * heads * 4;
+  plan.state_bytes = plan.max_full * (plan.parts + 1) * row;
+  plan.bytes = plan.state_bytes + plan.max_full * plan.parts * heads * 4;
   return plan;
 }
 
@@ -233,8 +244,8 @@ int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, void* wor
                   uint64_t workspace_bytes, cudaStream_t st) {
   if (int rc = scan_setup()) return rc;
   ScanPlan plan = scan_plan(seqs, p.tokens, p.heads, p.head_dim, state_dim);
-  if (!workspace || workspace_bytes < plan.bytes) plan = ScanPlan{};
-  if (plan.max_full + seqs > 65535) plan = ScanPlan{};
+  if (!workspace || workspace_bytes < plan.bytes || plan.max_full * plan.parts + seqs > 65535)
+    plan = ScanPlan{0, 1, 0, 0, 0};
   // Without tokens every sequence is empty and nothing is loaded; the maps still
   // need an extent, so they describe one token's worth of new_state.
   const bool some = p.tokens > 0;
@@ -254,12 +265,13 @@ int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, void* wor
   ScanParams sp{};
   sp.s = p;
   sp.seg_chunks = plan.seg_chunks;
+  sp.parts = plan.parts;
   sp.max_full = static_cast<int>(plan.max_full);
   sp.seg_state = static_cast<float*>(workspace);
   sp.seg_decay = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.state_bytes);
   const unsigned units = static_cast<unsigned>(p.heads * (p.head_dim / kScanCols));
   if (plan.max_full > 0) {
-    const dim3 pieces(units, static_cast<unsigned>(plan.max_full));
+    const dim3 pieces(units, static_cast<unsigned>(plan.max_full * plan.parts));
     if (state_dim == 64)
       gdn_ssm_piece_state_kernel<64><<<pieces, kStateThreads, kStateSmem, st>>>(tx, tb, sp);
     else
@@ -422,8 +434,10 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
   p.groups = num_groups;
   p.head_dim = head_dim;
   if (!A_log) return invalid("null pointer argument");
-  if (total_tokens > 0)
+  if (total_tokens > 0) {
     if (int rc = check_ssm_rows(p)) return rc;
+    if (!aligned(output, 32)) return invalid("output needs 32-byte alignment");
+  }
   if (int rc = lib_device(&p.status, &sms)) return rc;
   return ssm_scan_call(p, state_dim, num_seqs, workspace, workspace_bytes,
                        static_cast<cudaStream_t>(stream));

@@ -25,13 +25,15 @@
 // columns' block, L_t - L_s = (L_t - L_r) + (L_r - L_s), neither part positive,
 // so e^{L_t - L_s} step_s is a row factor times a column factor.
 //
-// Twenty warps with one role each, handing over through mbarriers:
-//   0 TMA, two stages of {C, B, X}       1 issues the products
-//   4-7 gates, and S -> M (thread = token row)
+// Twenty-eight warps with one role each, handing over through mbarriers:
+//   0-1 gates                              2 TMA, two stages of {C, B, X}
+//   3 issues the products                  4-7, 24-27 S -> M (thread = token row)
 //   8-11 the state in registers (thread = state row)
-//   12-15 outputs (thread = token row)   16-19 w X (thread = token row)
-// The products of a chunk are issued as dS, Yo, Yd, then S of the next chunk.
-// The next w X is made in registers while dS still reads the last one.
+//   12-15 outputs (thread = token row)     16-23 w X (thread = half a token row)
+// One warp of each four works on a quarter of the rows, and M's last rows are the
+// longest: the gates sit with the first two quarters.
+// The products of a chunk are issued as dS, Yo, S of the next chunk, Yd: M is then
+// made while dS and Yo run.
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
 // there, so nothing of them (not even a NaN) enters a product's sum.
 #pragma once
@@ -45,7 +47,7 @@ namespace gdn {
 
 constexpr int kScanQ = 128;
 constexpr int kScanCols = 64;            // columns of P per CTA
-constexpr int kScanThreads = 640;
+constexpr int kScanThreads = 896;
 constexpr uint32_t kScanTile = 16384;    // 128 rows x 64 bf16
 
 // Shared memory: two stages of C (two halves of N), B (two halves) and X, the
@@ -63,12 +65,12 @@ constexpr uint32_t kScanSmem = kScMisc + 256;     // 227 KiB: all there is
 // Tensor memory columns.
 constexpr uint32_t kTmS = 0, kTmM = 128, kTmYd = 192, kTmYo = 256, kTmDs = 320;
 
-// Registers per thread of the five warpgroups: together the 640 x 96 that the
-// block is launched with.
-constexpr int kScanLaunchRegs = 96;
-constexpr int kScanRegs[5] = {56, 88, 120, 88, 128};
-static_assert(kScanRegs[0] + kScanRegs[1] + kScanRegs[2] + kScanRegs[3] + kScanRegs[4] ==
-                  5 * kScanLaunchRegs && kScanThreads * kScanLaunchRegs <= 65536,
+// Registers per thread by role; together no more than the 896 x 72 that the block
+// is launched with.
+constexpr int kScanLaunchRegs = 72;
+constexpr int kRegsIssue = 48, kRegsM = 72, kRegsState = 120, kRegsOut = 80, kRegsScale = 56;
+static_assert(kRegsIssue + 2 * kRegsM + kRegsState + kRegsOut + 2 * kRegsScale <= 7 * kScanLaunchRegs &&
+                  kScanThreads * kScanLaunchRegs <= 65536,
               "as launched");
 
 template <int kRegs> __device__ __forceinline__ void scan_set_regs() {
@@ -138,21 +140,23 @@ __device__ __forceinline__ uint32_t split_pair(uint64_t& v) {
 }
 
 enum ScanBar {
-  kBFullX = 0, kBFullBC = 2, kBEmpty = 4, kBEmptyC0 = 6, kBGateFull = 8, kBGateEmpty = 10,
-  kBSFull = 12, kBMFull, kBYFull, kBYEmpty, kBXwFull, kBDsFull, kBDsEmpty, kBHFull, kBHEmpty,
-  kBGateSum, kBDrain, kBCount
+  kBFullX = 0, kBFullBC = 2, kBEmpty = 4, kBGateFull = 6, kBGateEmpty = 8, kBSFull = 10,
+  kBSEmpty, kBMFull, kBYFull, kBYEmpty, kBXwFull, kBDsFull, kBDsEmpty, kBHFull, kBHEmpty,
+  kBDrain, kBCount
 };
 
 // Long sequences run in pieces of seg_chunks chunks side by side: a first kernel
-// makes the state that each piece but a sequence's last adds by itself, and its
-// decay; the scan of a piece then starts from the sum of those before it.
+// makes the state that each part of a piece (`parts` of them, except in a
+// sequence's last piece) adds by itself, and its decay; the scan of a piece then
+// starts from the sum of those before it.
 struct ScanParams {
   SsmParams s;
-  int seg_chunks;      // chunks of a piece; 0: sequences are not divided
+  int seg_chunks;      // chunks of a piece, a multiple of parts; 0: sequences are not divided
+  int parts;
   int max_full;        // grid rows for whole pieces; the last piece of every sequence follows
-  float* seg_state;    // [2 max_full][H][P][N]: pieces' states, then carried states of
-                       // divided sequences (read in place of a state updated in place)
-  float* seg_decay;    // [max_full][H]: log2 of the pieces' decays
+  float* seg_state;    // [max_full (parts + 1)][H][P][N]: the parts' states, then carried states
+                       // of divided sequences (read in place of a state updated in place)
+  float* seg_decay;    // [max_full parts][H]: log2 of the parts' decays
 };
 
 struct ScanItem {
@@ -345,39 +349,38 @@ struct ScanGates {
   }
 };
 
-// Row `row` of w X, split exactly into three bf16 parts.
-__device__ __forceinline__ void scan_split_row(uint32_t (&part)[3][32], const uint8_t* x, int row,
+// kN groups of eight columns from group j0 of row `row` of w X, split exactly into
+// three bf16 tiles.  (Kept small: passes of 16 columns.)
+template <int kN>
+__device__ __forceinline__ void scan_scale_row(uint8_t* xw, const uint8_t* x, int row, int j0,
                                                float w) {
   const uint64_t w2 = pair(w, w);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint4 u = *reinterpret_cast<const uint4*>(x + sw128_off(row, j));
+#pragma unroll 2
+  for (int j = j0; j < j0 + kN; ++j) {
+    const uint32_t off = sw128_off(row, j);
+    const uint4 u = *reinterpret_cast<const uint4*>(x + off);
     const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+    uint32_t part[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint64_t v = mul2(unpack_pair(in[i]), w2);
-      part[0][4 * j + i] = split_pair(v);
-      part[1][4 * j + i] = split_pair(v);
-      part[2][4 * j + i] = pack_pair(v);
+      part[0][i] = split_pair(v);
+      part[1][i] = split_pair(v);
+      part[2][i] = pack_pair(v);
     }
-  }
-}
-
-__device__ __forceinline__ void scan_store_row(uint8_t* xw, const uint32_t (&part)[3][32], int row) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
 #pragma unroll
     for (int k = 0; k < 3; ++k)
-      *reinterpret_cast<uint4*>(xw + k * kScanTile + sw128_off(row, j)) =
-          make_uint4(part[k][4 * j], part[k][4 * j + 1], part[k][4 * j + 2], part[k][4 * j + 3]);
+      *reinterpret_cast<uint4*>(xw + k * kScanTile + off) =
+          make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
+  }
 }
 
 // A weight below this exponent, or a decay, is zero in fp32 whatever the rest.
 constexpr float kScanGone = -300.0f;
 
 // ------------------------------------------------ the states of pieces
-// One CTA per whole piece that is not its sequence's last, and 64 columns of a
-// head: the state it adds, sum over its tokens of e^{L_end - L_s} step_s B_s x_s^T,
+// One CTA per part of a whole piece that is not its sequence's last, and 64
+// columns of a head: the state it adds, sum over its tokens of e^{L_end - L_s} step_s B_s x_s^T,
 // in one accumulator.  Chunks run from the last to the first, so that weights
 // only need the decays already seen, and end where those leave nothing.
 constexpr int kStateThreads = 384;
@@ -425,16 +428,18 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_b);
   }
-  if (warp == 2) scan_item(sp, blockIdx.y, reinterpret_cast<ScanItem*>(smem + kSsItem));
+  const int part = blockIdx.y % sp.parts;
+  if (warp == 2) scan_item(sp, blockIdx.y / sp.parts, reinterpret_cast<ScanItem*>(smem + kSsItem));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const ScanItem& it = *reinterpret_cast<const ScanItem*>(smem + kSsItem);
-  const int nch = warp_uniform(it.seq < 0 || it.piece == it.pieces - 1 ? 0 : it.chunks);
+  const int nch = warp_uniform(it.seq < 0 || it.piece == it.pieces - 1 ? 0 : it.chunks / sp.parts);
+  const int c0 = warp_uniform(it.c0 + part * nch);
   const long long hbase = (static_cast<long long>(head) * p.head_dim + col0) * N;
   const long long per_slot = static_cast<long long>(p.heads) * p.head_dim * N;
   const uint32_t tmem = static_cast<uint32_t>(warp_uniform(static_cast<int>(*tmem_ptr)));
-  const int t_last = warp_uniform(it.t_begin + (it.c0 + nch - 1) * kScanQ);
+  const int t_last = warp_uniform(it.t_begin + (c0 + nch - 1) * kScanQ);
   const ScanSync sync{smem_u32(bars), abort_flag};
   // Chunk i of the order, from the end: false once the decays leave nothing of it.
   auto more = [&](int i) { return later[2 * (i & 1)] > kScanGone; };
@@ -492,7 +497,7 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
     umma_commit_elect(bars + kADone);
     mbar_wait(bars + kADone, 0);
   } else if (warp < 4) {
-    const int last = it.c0 + nch - 1;
+    const int last = c0 + nch - 1;
     ScanGates gates;
     gates.start(p, it.t_begin, it.len, head, warp - 2 < nch ? last - (warp - 2) : -1);
 #pragma unroll 1
@@ -532,10 +537,8 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
       sync.arrive(kAGateEmpty + st);
       if (!go) break;
       if (!sync.wait(kAFull + st, i >> 1, kStatusTmaTimeout)) break;
-      uint32_t part[3][32];
-      scan_split_row(part, smem + st * kSsStage + kSsX, row, w);
       if (i >= 2 && !sync.wait(kAXwEmpty + st, (i >> 1) - 1, kStatusMmaTimeout)) break;
-      scan_store_row(smem + kSsXw + st * 3 * kScanTile, part, row);
+      scan_scale_row<8>(smem + kSsXw + st * 3 * kScanTile, smem + st * kSsStage + kSsX, row, 0, w);
       fence_proxy_async_smem();
       sync.arrive(kAXwFull + st);
     }
@@ -557,8 +560,9 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
     // A state that is updated in place is kept for the first piece, which may
     // run after the last one has stored its result.
     const long long slot = slot_of(p.slots, p.slots_is64, it.seq, p.pool, p.status, false);
-    if (it.piece == 0 && p.state == p.new_state && slot >= 0) {
-      float* dst = sp.seg_state + (sp.max_full + it.first_row) * per_slot + hbase;
+    if (it.piece == 0 && part == 0 && p.state == p.new_state && slot >= 0) {
+      float* dst = sp.seg_state +
+                   (static_cast<long long>(sp.max_full) * sp.parts + it.first_row) * per_slot + hbase;
       for (int e = threadIdx.x - 128; e < kScanCols * N; e += kStateThreads - 128)
         dst[e] = p.state[slot * per_slot + hbase + e];
     }
@@ -584,12 +588,8 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kScMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kScMisc + 8 * kBCount);
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + kScMisc + 8 * kBCount + 4);
-  // per stage, the decay of each 32 tokens of the chunk
-  float* totals = reinterpret_cast<float*>(smem + kScMisc + 8 * kBCount + 8);   // [2][4]
-  auto chunk_total = [&](int st) {
-    return (totals[4 * st + 3] + totals[4 * st + 2]) + totals[4 * st + 1] + totals[4 * st];
-  };
-  static_assert(8 * kBCount + 40 <= 224 && sizeof(ScanItem) <= 32, "they fit");
+  float* totals = reinterpret_cast<float*>(smem + kScMisc + 8 * kBCount + 8);   // [2]
+  static_assert(8 * kBCount + 16 <= 224 && sizeof(ScanItem) <= 32, "they fit");
 
   if (warp == 0) {
     tmem_alloc(tmem_ptr, 512);
@@ -601,10 +601,10 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     for (int i = 0; i < kBCount; ++i) {
       int n = 1;
       if (i == kBEmpty || i == kBEmpty + 1) n = 1 + 4;   // products, output warps
-      else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 16;
-      else if (i == kBEmptyC0 || i == kBEmptyC0 + 1 || i == kBMFull || i == kBYEmpty ||
-               i == kBXwFull || i == kBHFull || i == kBDsEmpty || i == kBGateFull || i == kBGateFull + 1 ||
-               i == kBGateSum)
+      else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 24;
+      else if (i == kBXwFull || i == kBMFull || i == kBSEmpty) n = 8;
+      else if (i == kBYEmpty ||
+               i == kBHFull || i == kBDsEmpty)
         n = 4;
       mbar_init(bars + i, n);
     }
@@ -650,11 +650,9 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         }
     }
   } else if (warp < 4) {
-    scan_set_regs<kScanRegs[0]>();
-    if (warp == 0) {
+    scan_set_regs<kRegsIssue>();
+    if (warp == 2) {
       // ---------------------------------------------- TMA
-      // C's first half is the last part of a stage to come free: the outputs
-      // pass through it.
       int issued = 0;
       bool ok = true;
 #pragma unroll 1
@@ -669,23 +667,20 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
           uint64_t* bar = bars + kBFullBC + st;
           mbar_arrive_expect_tx(bar, 2 * (N / 64) * kScanTile);
 #pragma unroll
-          for (int b = 0; b < N / 64; ++b)
+          for (int b = 0; b < N / 64; ++b) {
             tma_load_3d(stage + kScB + b * kScanTile, &tm_b, bar, 64 * b, group, t0);
-          if constexpr (N == 128) tma_load_3d(stage + kScC + kScanTile, &tm_c, bar, 64, group, t0);
+            tma_load_3d(stage + kScC + b * kScanTile, &tm_c, bar, 64 * b, group, t0);
+          }
         }
         __syncwarp();
         issued = c + 1;
-        if (c >= 2) ok = wait(kBEmptyC0 + st, (c >> 1) - 1, kStatusMmaTimeout);
-        if (elect_one()) tma_load_3d(stage + kScC, &tm_c, bars + kBFullBC + st, 0, group, t0);
-        __syncwarp();
-        if (!ok) break;
       }
       if (!ok)   // aborted: the copies in flight land first
         for (int c = max(issued - 2, 0); c < issued; ++c) {
           mbar_wait(bars + kBFullX + (c & 1), (c >> 1) & 1);
           mbar_wait(bars + kBFullBC + (c & 1), (c >> 1) & 1);
         }
-    } else if (warp == 1) {
+    } else if (warp == 3) {
       // ---------------------------------------------- products
       // Every lane runs the whole sequence and an elected one issues: the warp
       // never diverges, so descriptors stay in uniform registers.  (Inside a
@@ -700,11 +695,10 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       bool ok = true;
 #pragma unroll 1
       for (int c = -1; c < nch; ++c) {
+        const uint32_t st = base + (c & 1) * kScStage;
         if (c >= 0) {
-          const uint32_t st = base + (c & 1) * kScStage;
           const uint64_t bt_desc = sdesc_sw128(st + kScB, kScanTile, 1024);
           const uint64_t c_desc = sdesc_sw128(st + kScC, 16, 1024);
-          const uint64_t x_desc = sdesc_sw128(st + kScX, kScanTile, 1024);
           if (!(ok = wait(kBXwFull, c, kStatusMmaTimeout))) break;
           if (c > 0 && !(ok = wait(kBDsEmpty, c - 1, kStatusMmaTimeout))) break;
           tc_fence_after();
@@ -721,6 +715,23 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             umma_bf16_elect(tmem + kTmYo, sdesc_add(c_desc, (s >> 2) * kScanTile + (s & 3) * 32),
                             sdesc_add(h_desc, s * 2048), idesc_y, s > 0);
           umma_commit_elect(bars + kBHEmpty);
+        }
+        if (c + 1 < nch) {
+          const uint32_t next = base + ((c + 1) & 1) * kScStage;
+          const uint64_t c_desc = sdesc_sw128(next + kScC, 16, 1024);
+          const uint64_t b_desc = sdesc_sw128(next + kScB, 16, 1024);
+          if (!(ok = wait(kBFullBC + ((c + 1) & 1), (c + 1) >> 1, kStatusTmaTimeout))) break;
+          if (c >= 0 && !(ok = wait(kBSEmpty, c, kStatusMmaTimeout))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const uint32_t off = (s >> 2) * kScanTile + (s & 3) * 32;
+            umma_bf16_elect(tmem + kTmS, sdesc_add(c_desc, off), sdesc_add(b_desc, off), idesc_s, s > 0);
+          }
+          umma_commit_elect(bars + kBSFull);
+        }
+        if (c >= 0) {
+          const uint64_t x_desc = sdesc_sw128(st + kScX, kScanTile, 1024);
           if (!(ok = wait(kBMFull, c, kStatusMmaTimeout))) break;
           tc_fence_after();
 #pragma unroll
@@ -730,117 +741,95 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
           umma_commit_elect(bars + kBYFull);
           if (c + 2 < nch) umma_commit_elect(bars + kBEmpty + (c & 1));
         }
-        if (c + 1 < nch) {   // M of this chunk is made, so S is read
-          const uint32_t st = base + ((c + 1) & 1) * kScStage;
-          const uint64_t c_desc = sdesc_sw128(st + kScC, 16, 1024);
-          const uint64_t b_desc = sdesc_sw128(st + kScB, 16, 1024);
-          if (!(ok = wait(kBFullBC + ((c + 1) & 1), (c + 1) >> 1, kStatusTmaTimeout))) break;
-          tc_fence_after();
-#pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            const uint32_t off = (s >> 2) * kScanTile + (s & 3) * 32;
-            umma_bf16_elect(tmem + kTmS, sdesc_add(c_desc, off), sdesc_add(b_desc, off), idesc_s, s > 0);
-          }
-          umma_commit_elect(bars + kBSFull);
-        }
       }
       if (!ok) {   // aborted: the products in flight finish first
         umma_commit_elect(bars + kBDrain);
         mbar_wait(bars + kBDrain, 0);
       }
-    }
-  } else if (warp < 8) {
-    // ------------------------------------------------ S -> M
-    scan_set_regs<kScanRegs[1]>();
-    // The gates, thread = token: a suffix sum over the chunk in the warp, and over
-    // the four warps through shared memory.  Those of the next chunk are made
-    // while this one's S is.
-    const float a2 = -expf(p.A_log[head]) * 1.4426950408889634f;
-    const float bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
-    const __nv_bfloat16* dt = p.dt + t_begin * p.dt_stride + head;
-    __nv_bfloat16 raw = __float2bfloat16_rn(0.0f);
-    if (row < len) raw = dt[row * p.dt_stride];
-    auto make_gates = [&](int c) {
-      const int st = c & 1, t = c * kScanQ + row;
-      float step = scan_step_size(to_float(raw) + bias);
-      if (t >= len) step = 0.0f;
-      if (t + kScanQ < len) raw = dt[(t + kScanQ) * p.dt_stride];
-      float v = a2 * step;
+    } else {
+      // ---------------------------------------------- gates
+      // Two warps take turns; a chunk's dt are on their way while the chunk
+      // before it (of this warp) is worked on.
+      ScanGates gates;
+      gates.start(p, t_begin, len, head, warp);
+#pragma unroll 1
+      for (int c = warp; c < nch; c += 2) {
+        const int st = c & 1;
+        gates.make(c, c + 2);
+        if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) break;
+        float* g = reinterpret_cast<float*>(smem + kScGate + st * kScGateStage) + lane;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {   // sums over this lane and those after it
-        const float u = __shfl_down_sync(0xffffffffu, v, o);
-        if (lane + o < 32) v += u;
+        for (int b = 0; b < 4; ++b) {
+          // log2 of a zero step is -inf: a padded token has no weight anywhere
+          g[32 * b] = gates.sfx[b] + scan_log2(gates.step[b]);
+          g[kScanQ + 32 * b] = gates.sfx[b];
+          if (b < 3) g[2 * kScanQ + 32 * b] = gates.step[b] * scan_exp2(gates.sfx[b] - gates.ref[b]);
+        }
+        if (lane == 0) totals[st] = gates.total;
+        arrive(kBGateFull + st);
       }
-      float sfx = __shfl_down_sync(0xffffffffu, v, 1);
-      if (lane == 31) sfx = 0.0f;
-      if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) return false;
-      float* g = reinterpret_cast<float*>(smem + kScGate + st * kScGateStage);
-      float* sums = totals + 4 * st;
-      if (lane == 0) sums[quad] = v;
-      arrive(kBGateSum);
-      if (!wait(kBGateSum, c, kStatusMmaTimeout)) return false;
-      const float before_last = sfx;
-      float ref = 0.0f;                    // decays of the blocks after this one
-      for (int b = 3; b > quad; --b) ref += sums[b];
-      sfx += ref;
-      // log2 of a zero step is -inf: a padded token has no weight anywhere
-      g[row] = sfx + scan_log2(step);
-      g[kScanQ + row] = sfx;
-      if (quad < 3) g[2 * kScanQ + row] = step * scan_exp2(before_last);
-      arrive(kBGateFull + st);
-      return true;
-    };
-    bool ok = make_gates(0);
-    {   // blocks above the diagonal stay zero
+    }
+  } else if (warp < 8 || warp >= 24) {
+    // ------------------------------------------------ S -> M
+    // The row quarter's 32 x 32 blocks up to the diagonal one: that one and every
+    // second before it by the first warpgroup, the rest by the other.
+    scan_set_regs<kRegsM>();
+    const int top = warp < 8 ? quad : quad - 1;
+    if (warp < 8) {   // blocks above the diagonal stay zero
       const uint32_t z[16] = {};
+#pragma unroll 1
       for (int b = quad + 1; b < 4; ++b) tmem_st16(tmem + kTmM + 16 * b + tm_lane, z);
       tmem_wait_st();
     }
 #pragma unroll 1
-    for (int c = 0; ok && c < nch; ++c) {
+    for (int c = 0; c < nch; ++c) {
       const int st = c & 1;
-      if (c + 1 < nch && !make_gates(c + 1)) break;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
       const float* g = reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage);
       const float mine = g[kScanQ + row];
-      if (!wait(kBSFull, c, kStatusMmaTimeout)) break;   // also: the last M is read
+      if (!wait(kBSFull, c, kStatusMmaTimeout)) break;
       tc_fence_after();
+      bool ok = true;
 #pragma unroll 1
-      for (int b = 0; b < quad; ++b) {
+      for (int b = top; b >= 0 && ok; b -= 2) {
         float s[32];
+        uint32_t m[16];
         tmem_ld32(tmem + kTmS + 32 * b + tm_lane, s);
-        const float u = scan_exp2(g[kScanQ + 32 * b + 31] - mine);
-        const uint64_t u2 = pair(u, u);
-        const float4* v = reinterpret_cast<const float4*>(g + 2 * kScanQ + 32 * b);
-        uint32_t m[16];
-        tmem_wait_ld();
+        if (b == quad) {
+          const float4* f4 = reinterpret_cast<const float4*>(g + 32 * b);
+          tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 f = v[j];
-          m[2 * j] = pack_pair(mul2(mul2(pair(s[4 * j], s[4 * j + 1]), u2), pair(f.x, f.y)));
-          m[2 * j + 1] = pack_pair(mul2(mul2(pair(s[4 * j + 2], s[4 * j + 3]), u2), pair(f.z, f.w)));
+          for (int j = 0; j < 8; ++j) {
+            const float4 gv = f4[j];
+            const float f[4] = {gv.x, gv.y, gv.z, gv.w};
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)   // a select: a masked S may hold anything
+              v[e] = 4 * j + e <= lane ? s[4 * j + e] * scan_exp2(f[e] - mine) : 0.0f;
+            m[2 * j] = pack_bf16x2(v[0], v[1]);
+            m[2 * j + 1] = pack_bf16x2(v[2], v[3]);
+          }
+        } else {
+          const float u = scan_exp2(g[kScanQ + 32 * b + 31] - mine);
+          const uint64_t u2 = pair(u, u);
+          const float4* v = reinterpret_cast<const float4*>(g + 2 * kScanQ + 32 * b);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 f = v[j];
+            m[2 * j] = pack_pair(mul2(mul2(pair(s[4 * j], s[4 * j + 1]), u2), pair(f.x, f.y)));
+            m[2 * j + 1] = pack_pair(mul2(mul2(pair(s[4 * j + 2], s[4 * j + 3]), u2), pair(f.z, f.w)));
+          }
         }
-        tmem_st16(tmem + kTmM + 16 * b + tm_lane, m);
-      }
-      {
-        float s[32];
-        tmem_ld32(tmem + kTmS + 32 * quad + tm_lane, s);
-        const float4* f4 = reinterpret_cast<const float4*>(g + 32 * quad);
-        uint32_t m[16];
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 gv = f4[j];
-          const float f[4] = {gv.x, gv.y, gv.z, gv.w};
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)   // a select: a masked S may hold anything
-            v[e] = 4 * j + e <= lane ? s[4 * j + e] * scan_exp2(f[e] - mine) : 0.0f;
-          m[2 * j] = pack_bf16x2(v[0], v[1]);
-          m[2 * j + 1] = pack_bf16x2(v[2], v[3]);
+        if (b < 2) {   // the last of S is read
+          tc_fence_before();
+          arrive(kBSEmpty);
         }
-        tmem_st16(tmem + kTmM + 16 * quad + tm_lane, m);
+        if (b == top && c > 0) ok = wait(kBYFull, c - 1, kStatusMmaTimeout);   // the last M is read
+        if (ok) tmem_st16(tmem + kTmM + 16 * b + tm_lane, m);
       }
+      if (!ok) break;
+      if (top < 0) arrive(kBSEmpty);
       tmem_wait_st();
       tc_fence_before();
       arrive(kBMFull);
@@ -848,7 +837,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     }
   } else if (warp < 12) {
     // ------------------------------------------------ the state
-    scan_set_regs<kScanRegs[2]>();
+    scan_set_regs<kRegsState>();
     const bool state_row = row < N;
     uint64_t h[kScanCols / 2];
 #pragma unroll
@@ -866,16 +855,18 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     const long long slot = find_state(carried);
     if (state_row) {   // the start: what the pieces before this one leave, and the carried state
       float log_decay = 0.0f;
+      const long long row0 = static_cast<long long>(it.first_row) * sp.parts;
 #pragma unroll 1
-      for (int r = it.piece - 1; r >= (carried ? -1 : 0) && log_decay > kScanGone; --r) {
-        const float* src = sp.seg_state + (it.first_row + r) * per_slot + hbase;
+      for (int r = it.piece * sp.parts - 1; r >= (carried ? -1 : 0) && log_decay > kScanGone; --r) {
+        const float* src = sp.seg_state + (row0 + r) * per_slot + hbase;
         if (r < 0)
           src = it.pieces > 1 && p.state == p.new_state
-                    ? sp.seg_state + (sp.max_full + it.first_row) * per_slot + hbase
+                    ? sp.seg_state +
+                          (static_cast<long long>(sp.max_full) * sp.parts + it.first_row) * per_slot + hbase
                     : p.state + slot * per_slot + hbase;
         add_state(src, log_decay);
         if (r >= 0)
-          log_decay += sp.seg_decay[static_cast<long long>(it.first_row + r) * p.heads + head];
+          log_decay += sp.seg_decay[(row0 + r) * p.heads + head];
       }
     }
     bool ok = true;
@@ -893,7 +884,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       fence_proxy_async_smem();
       arrive(kBHFull);
       if (!(ok = wait(kBGateFull + st, c >> 1, kStatusMmaTimeout))) break;
-      const float decay = scan_exp2(chunk_total(st));
+      const float decay = scan_exp2(totals[st]);
       const uint64_t d2 = pair(decay, decay);
       arrive(kBGateEmpty + st);
       if (!(ok = wait(kBDsFull, c, kStatusMmaTimeout))) break;
@@ -925,9 +916,10 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         dst[(2 * j + 1) * N] = f.y;
       }
     }
-  } else if (warp >= 16) {
+  } else if (warp >= 16 && warp < 24) {
     // ------------------------------------------------ w X
-    scan_set_regs<kScanRegs[4]>();
+    scan_set_regs<kRegsScale>();
+    const int j0 = (warp - 16) >> 2 << 2;   // groups of eight columns
 #pragma unroll 1
     for (int c = 0; c < nch; ++c) {
       const int st = c & 1, n = chunk_len(c);
@@ -940,7 +932,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         if (!wait(kBFullBC + st, c >> 1, kStatusTmaTimeout)) break;
         if (row >= n) {
 #pragma unroll 1
-          for (int j = 0; j < 8; ++j) {
+          for (int j = j0; j < j0 + 4; ++j) {
             const uint32_t off = sw128_off(row, j);
             const uint4 z = make_uint4(0u, 0u, 0u, 0u);
             *reinterpret_cast<uint4*>(stage + kScX + off) = z;
@@ -950,16 +942,14 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
           }
         }
       }
-      uint32_t part[3][32];
-      scan_split_row(part, stage + kScX, row, w);
       if (c > 0 && !wait(kBDsFull, c - 1, kStatusMmaTimeout)) break;   // the last w X is read
-      scan_store_row(smem + kScXw, part, row);
+      scan_scale_row<4>(smem + kScXw, stage + kScX, row, j0, w);
       fence_proxy_async_smem();
       arrive(kBXwFull);
     }
   } else {
     // ------------------------------------------------ outputs
-    scan_set_regs<kScanRegs[3]>();
+    scan_set_regs<kRegsOut>();
     const float D = p.D ? p.D[head] : 0.0f;
     const uint64_t D2 = pair(D, D);
 #pragma unroll 1
@@ -968,7 +958,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       uint8_t* stage = smem + st * kScStage;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
       const float e = scan_exp2(
-          chunk_total(st) - reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row]);
+          totals[st] - reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row]);
       arrive(kBGateEmpty + st);
       if (!wait(kBFullX + st, c >> 1, kStatusTmaTimeout)) break;
       uint4 x[8];   // kept here so that the stage can be refilled early
@@ -978,43 +968,34 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       arrive(kBEmpty + st);
       if (!wait(kBYFull, c, kStatusMmaTimeout)) break;
       tc_fence_after();
-      // the row's results go to C's first half in shared memory (no product
-      // reads it any more), from where the warp writes whole rows
+      // 32 bytes of the thread's row at a time, whole sectors: no detour through
+      // shared memory, which would hold up the stage
       const uint64_t e2 = pair(e, e);
+      __nv_bfloat16* out = p.out +
+          ((static_cast<long long>(t_begin) + c * kScanQ + row) * p.heads + head) * p.head_dim + col0;
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) {   // 16 columns at a time
+      for (int b = 0; b < 4; ++b) {
         uint32_t yd[16], yo[16];
         tmem_ld16(tmem + kTmYd + 16 * b + tm_lane, yd);
         tmem_ld16(tmem + kTmYo + 16 * b + tm_lane, yo);
         tmem_wait_ld();
         const uint32_t in[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-        uint32_t out[8];
+        uint32_t y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          out[i] = pack_pair(fma2(D2, unpack_pair(in[i]),
-                                  fma2(e2, pair_bits(yo[2 * i], yo[2 * i + 1]),
-                                       pair_bits(yd[2 * i], yd[2 * i + 1]))));
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          *reinterpret_cast<uint4*>(stage + kScC + sw128_off(row, 2 * b + j)) =
-              make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
+          y[i] = pack_pair(fma2(D2, unpack_pair(in[i]),
+                                fma2(e2, pair_bits(yo[2 * i], yo[2 * i + 1]),
+                                     pair_bits(yd[2 * i], yd[2 * i + 1]))));
+        if (row < n)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + 16 * b),
+                       "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]),
+                       "r"(y[7])
+                       : "memory");
 #pragma unroll
         for (int j = 0; j < 6; ++j) x[j] = x[j + 2];
       }
       tc_fence_before();
       arrive(kBYEmpty);
-      __syncwarp();
-      __nv_bfloat16* out = p.out +
-          ((static_cast<long long>(t_begin) + c * kScanQ) * p.heads + head) * p.head_dim + col0;
-      const long long ld = static_cast<long long>(p.heads) * p.head_dim;
-#pragma unroll 2
-      for (int i = 0; i < 8; ++i) {
-        const int r = quad * 32 + 4 * i + (lane >> 3);
-        const uint4 u = *reinterpret_cast<const uint4*>(stage + kScC + sw128_off(r, lane & 7));
-        if (r < n) *reinterpret_cast<uint4*>(out + r * ld + 8 * (lane & 7)) = u;
-      }
-      fence_proxy_async_smem();   // the next copy into this half comes after these accesses
-      arrive(kBEmptyC0 + st);
     }
   }
   tc_fence_before();
