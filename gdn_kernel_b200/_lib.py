@@ -15,6 +15,7 @@ import threading
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libgdn_b200.so")
 TVM_DECODE_PATH = os.path.join(_PKG, "libgdn_b200_tvm_decode.so")
+TVM_MIXER_PATH = os.path.join(_PKG, "libgdn_b200_tvm_mixer.so")
 TVM_PREFILL_PATH = os.path.join(_PKG, "libgdn_b200_tvm_prefill.so")
 
 GDN_B200_OK = 0

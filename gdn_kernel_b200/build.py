@@ -3,6 +3,7 @@
 * ``libgdn_b200.so``           — CUDA kernels + the C ABI of ``include/gdn_b200.h``
 * ``libgdn_b200_tvm_decode.so``  — TVM-FFI ``kernel`` export for decode
 * ``libgdn_b200_tvm_prefill.so`` — TVM-FFI ``kernel`` export for prefill
+* ``libgdn_b200_tvm_mixer.so``   — TVM-FFI exports of the mixer operators
 
 Run ``python -m gdn_kernel_b200.build`` from the repository root.  nvcc
 cross-compiles without a GPU; the outputs sit next to this file so that they
@@ -29,6 +30,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
 LIB = os.path.join(PKG, "libgdn_b200.so")
 TVM_DECODE = os.path.join(PKG, "libgdn_b200_tvm_decode.so")
 TVM_PREFILL = os.path.join(PKG, "libgdn_b200_tvm_prefill.so")
+TVM_MIXER = os.path.join(PKG, "libgdn_b200_tvm_mixer.so")
 
 
 def _nvcc() -> str:
@@ -92,7 +94,8 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
     tvm_inc = libinfo.find_include_path()
     dl_inc = libinfo.find_dlpack_include_path()
     tvm_lib = os.path.dirname(libinfo.find_libtvm_ffi())
-    for target, src in ((TVM_DECODE, "tvm_ffi_decode.cc"), (TVM_PREFILL, "tvm_ffi_prefill.cc")):
+    for target, src in ((TVM_DECODE, "tvm_ffi_decode.cc"), (TVM_PREFILL, "tvm_ffi_prefill.cc"),
+                        (TVM_MIXER, "tvm_ffi_mixer.cc")):
         deps = _sources(src, "tvm_ffi_common.h") + [os.path.join(INCLUDE, "gdn_b200.h"), LIB]
         if force or _stale(target, deps):
             cuda = os.path.dirname(os.path.dirname(_nvcc()))

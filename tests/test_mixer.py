@@ -77,33 +77,103 @@ def test_nothing_to_do_is_no_error(fn, kw):
     assert lib.gdn_b200_last_error() == b""
 
 
-def test_python_refuses_cpu_tensors():
-    x = torch.zeros(4, 64, dtype=torch.bfloat16)
-    w = torch.zeros(64, 4, dtype=torch.bfloat16)
-    cu = torch.tensor([0, 4], dtype=torch.int32)
-    for call in (lambda: M.gdn_short_conv(x, w, None, None, cu, x, None),
-                 lambda: M.gdn_short_conv_step(x, w, None, x, None, x),
-                 lambda: M.gdn_ssm_prefill(x, x, None, x, x, None, None, None, cu, x, x),
-                 lambda: M.gdn_ssm_step(x, x, None, x, x, None, None, x, None, x),
-                 lambda: M.gdn_gated_norm(x, x, None, x),
-                 lambda: M.gdn_add_norm(x, x, x, x, x)):
-        with pytest.raises(ValueError, match="CUDA"):
-            call()
+BF = torch.bfloat16
 
 
-@pytest.mark.parametrize("shape,name", [((3, 64), "shape"), ((4, 60), "shape")])
-def test_row_checks_name_the_operand(shape, name):
-    t = torch.zeros(4, 64)
-    with pytest.raises(ValueError, match="x: expected shape"):
-        M._rows(t, "x", torch.float32, shape, t.device)
-    with pytest.raises(ValueError, match="x: expected torch.bfloat16"):
-        M._rows(t, "x", torch.bfloat16, (4, 64), t.device)
-    with pytest.raises(ValueError, match="contiguous within a row"):
-        M._rows(t.t(), "x", torch.float32, (64, 4), t.device)
-    assert M._rows(t[:, :60], "x", torch.float32, (4, 60), t.device)[1] == 64
-    assert M._rows(t.view(4, 8, 8)[:, :4], "x", torch.float32, (4, 4, 8), t.device)[1] == 64
-    with pytest.raises(ValueError, match="contiguous within a row"):
-        M._rows(t.view(4, 8, 8)[:, :, :4], "x", torch.float32, (4, 8, 4), t.device)
+def z(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype)
+
+
+CU = torch.tensor([0, 4], dtype=torch.int32)
+
+
+def conv(x=z(4, 64), weight=z(64, 4), bias=None, state=None, cu=CU, output=z(4, 64),
+         new_state=z(1, 3, 64), **kw):
+    M.gdn_short_conv(x, weight, bias, state, cu, output, new_state, **kw)
+
+
+def conv_step(x=z(4, 64), weight=z(64, 4), bias=None, state_pool=z(4, 3, 64), slots=None,
+              output=z(4, 64), **kw):
+    M.gdn_short_conv_step(x, weight, bias, state_pool, slots, output, **kw)
+
+
+def scan(x=z(4, 2, 64), dt=z(4, 2), A_log=z(2, dtype=torch.float32), B=z(4, 1, 128),
+         C=z(4, 1, 128), D=None, dt_bias=None, state=None, cu=CU, output=z(4, 2, 64),
+         new_state=z(1, 2, 64, 128, dtype=torch.float32), **kw):
+    M.gdn_ssm_prefill(x, dt, A_log, B, C, D, dt_bias, state, cu, output, new_state, **kw)
+
+
+def scan_step(x=z(4, 2, 64), dt=z(4, 2), A_log=z(2, dtype=torch.float32), B=z(4, 1, 128),
+              C=z(4, 1, 128), D=None, dt_bias=None, pool=z(4, 2, 64, 128, dtype=torch.float32),
+              slots=None, output=z(4, 2, 64), **kw):
+    M.gdn_ssm_step(x, dt, A_log, B, C, D, dt_bias, pool, slots, output, **kw)
+
+
+def gated(x=z(4, 64), gate=z(4, 64), weight=z(64), output=z(4, 64), **kw):
+    M.gdn_gated_norm(x, gate, weight, output, **kw)
+
+
+def add(x=z(4, 64), residual=z(4, 64), weight=z(64), output=z(4, 64), new_residual=z(4, 64), **kw):
+    M.gdn_add_norm(x, residual, weight, output, new_residual, **kw)
+
+
+F32, I32, I64 = torch.float32, torch.int32, torch.int64
+
+
+@pytest.mark.parametrize("call,kw,words", [
+    # what is right but not on a GPU, last of all checks
+    (conv, {}, "CUDA"), (conv_step, {}, "CUDA"), (scan, {}, "CUDA"), (scan_step, {}, "CUDA"),
+    (gated, {}, "CUDA"), (add, {}, "CUDA"),
+    (gated, dict(x=z(4, 130)[:, :64], gate=z(4, 72)[:, :64]), "CUDA"),     # row strides are free
+    (scan, dict(x=z(4, 200)[:, :128].view(4, 2, 64), D=z(2, dtype=F32)), "CUDA"),
+    # types
+    (conv, dict(x=z(4, 64, dtype=torch.int32)), "x: expected bfloat16"),
+    (conv, dict(weight=z(64, 4, dtype=F32)), "weight: wrong dtype"),
+    (conv, dict(state=z(1, 3, 64, dtype=F32)), "state: wrong dtype"),
+    (conv, dict(cu=CU.float()), "cu_seqlens: must be int32 or int64"),
+    (conv, dict(state_indices=z(1, dtype=F32)), "state_indices: must be"),
+    (conv, dict(has_state=z(1, dtype=I32)), "has_state: must be bool or uint8"),
+    (scan, dict(x=z(4, 2, 64, dtype=F32)), "x: wrong dtype"),
+    (scan, dict(A_log=z(2)), "A_log: wrong dtype"), (scan, dict(dt=z(4, 2, dtype=F32)), "dt"),
+    (scan_step, dict(slots=torch.arange(4), output_state_indices=torch.arange(4, dtype=I32)),
+     "output_state_indices"),
+    (gated, dict(weight=z(64, dtype=F32)), "weight: wrong dtype"),
+    (add, dict(residual=z(4, 64, dtype=torch.float16)), "residual"),
+    (add, dict(residual=z(4, 64, dtype=F32)), "new_residual: wrong dtype"),
+    (add, dict(scale=z(64)), "scale: wrong dtype"),
+    # shapes
+    (conv, dict(weight=z(64, 5)), "width"), (conv, dict(weight=z(64)), "weight"),
+    (conv, dict(x=z(4, 60)), "x: expected shape \\(4, 64\\), got \\(4, 60\\)"),
+    (conv, dict(output=z(5, 64)), "output: expected shape"), (conv, dict(bias=z(63)), "bias"),
+    (conv, dict(new_state=z(1, 2, 64)), "new_state"), (conv, dict(new_state=z(64)), "new_state"),
+    (conv, dict(new_state=z(0, 3, 64)), "0 rows, 1 are needed"),
+    (conv, dict(cu=z(1, 2, dtype=I32)), "cu_seqlens"),
+    (conv, dict(state_indices=z(2, dtype=I64)), "state_indices: expected shape"),
+    (conv, dict(x=z(4, 8, 8)), "two dimensions"),
+    (conv_step, dict(state_pool=z(3, 3, 64)), "3 rows, 4 are needed"),
+    (conv_step, dict(new_state_pool=z(3, 3, 64)), "new_state_pool"),
+    (scan, dict(x=z(4, 2, 96), output=z(4, 2, 96)), "head_dim"), (scan, dict(x=z(4, 128)), "x"),
+    (scan, dict(B=z(4, 1, 32)), "state_dim"), (scan, dict(C=z(4, 1, 64)), "C: expected shape"),
+    (scan, dict(x=z(4, 3, 64), B=z(4, 2, 128)), "multiple"), (scan, dict(D=z(3, dtype=F32)), "D"),
+    (scan, dict(dt=z(3, 2)), "dt"), (scan, dict(new_state=z(1, 2, 64, dtype=F32)), "new_state"),
+    (scan_step, dict(pool=z(3, 2, 64, 128, dtype=F32)), "3 rows, 4 are needed"),
+    (gated, dict(group_size=48), "divide"), (gated, dict(group_size=0), "group_size"),
+    (gated, dict(weight=z(32)), "weight: expected"), (gated, dict(gate=z(4, 32)), "gate"),
+    (gated, dict(x=z(64)), "must be"), (add, dict(weight=z(63)), "weight"),
+    (add, dict(x=z(4, 0)), "empty"), (add, dict(block_weight=z(63)), "block_weight"),
+    # layouts
+    (conv, dict(x=z(64, 4).t()), "x: must be contiguous within a row"),
+    (conv, dict(state=z(1, 64, 3).transpose(1, 2)), "state: must be contiguous"),
+    (scan, dict(x=z(4, 2, 128)[:, :, ::2]), "x: must be contiguous within a row"),
+    (scan, dict(B=z(4, 256).view(4, 2, 128)[:, ::2]), "CUDA"),
+    (gated, dict(weight=z(128)[::2]), "weight: must be contiguous"),
+    (add, dict(output=z(4, 128)[:, ::2]), "output: must be contiguous within a row"),
+    # words
+    (conv, dict(activation="sigmoid"), "activation"), (gated, dict(activation=None), "activation"),
+])
+def test_python_refuses(call, kw, words):
+    with pytest.raises(ValueError, match=words):
+        call(**kw)
 
 
 # ------------------------------------------------------------------ the oracle
