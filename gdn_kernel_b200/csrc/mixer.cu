@@ -39,39 +39,52 @@ bool wide_rows(const void* p, long long stride, int size) {
 
 // ------------------------------------------------------------ short convolution
 template <typename T, int V, int W>
-void launch_conv(ConvParams& p, long long blocks_per_chan, bool step, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>(blocks_per_chan * p.chan_blocks);
+void launch_conv(const ConvParams& p, bool step, cudaStream_t st) {
+  constexpr unsigned per_block = kConvThreads / 32;
+  const unsigned grid = (p.warps + per_block - 1) / per_block;
   if (step) gdn_short_conv_step_kernel<T, V, W><<<grid, kConvThreads, 0, st>>>(p);
   else gdn_short_conv_kernel<T, V, W><<<grid, kConvThreads, 0, st>>>(p);
 }
 
 template <typename T, int V>
-void launch_conv_width(ConvParams& p, int width, long long n, bool step, cudaStream_t st) {
-  if (width == 2) launch_conv<T, V, 2>(p, n, step, st);
-  else if (width == 3) launch_conv<T, V, 3>(p, n, step, st);
-  else launch_conv<T, V, 4>(p, n, step, st);
+void launch_conv_width(const ConvParams& p, int width, bool step, cudaStream_t st) {
+  if (width == 2) launch_conv<T, V, 2>(p, step, st);
+  else if (width == 3) launch_conv<T, V, 3>(p, step, st);
+  else launch_conv<T, V, 4>(p, step, st);
 }
 
+// Tokens of a warp: long ones re-read fewer rows before their first (W - 1 each)
+// and load their taps less often; short ones spread a small call over the SMs.
+constexpr int kConvTileLong = 32, kConvTileShort = 8;
+constexpr long long kConvFewWarps = 148 * 32;
+
 template <typename T>
-int launch_conv_type(ConvParams& p, int width, long long n, bool step, cudaStream_t st) {
+int launch_conv_type(ConvParams& p, int width, bool step, cudaStream_t st) {
   const int size = static_cast<int>(sizeof(T));
   // 16-byte vectors where every row starts on one, else one channel per thread
   const bool wide = p.channels % kLanes<T> == 0 && wide_rows(p.x, p.x_stride, size) &&
                     wide_rows(p.out, p.out_stride, size) && aligned(p.weight, 16) &&
                     aligned(p.bias, 16) && aligned(p.state, 16) && aligned(p.new_state, 16);
   const int v = wide ? kLanes<T> : 1;
-  p.chan_blocks = (p.channels / v + kConvThreads - 1) / kConvThreads;
-  if (n > kMaxGrid / p.chan_blocks) return invalid("tokens * channels exceeds the grid limit");
-  if (wide) launch_conv_width<T, kLanes<T>>(p, width, n, step, st);
-  else launch_conv_width<T, 1>(p, width, n, step, st);
+  p.chan_warps = (p.channels / v + 31) / 32;
+  long long n = p.tokens;   // rows of a step
+  if (!step) {
+    p.tile = (p.tokens / kConvTileLong + 1) * p.chan_warps < kConvFewWarps ? kConvTileShort
+                                                                         : kConvTileLong;
+    n = std::max<long long>(1, (p.tokens + p.tile - 1) / p.tile);
+  }
+  if (n > kMaxGrid / p.chan_warps) return invalid("tokens * channels exceeds the grid limit");
+  p.warps = static_cast<unsigned>(n * p.chan_warps);
+  if (wide) launch_conv_width<T, kLanes<T>>(p, width, step, st);
+  else launch_conv_width<T, 1>(p, width, step, st);
   return launched("short convolution launch");
 }
 
-int conv_call(ConvParams& p, int width, int32_t dtype, long long n, bool step, void* stream) {
+int conv_call(ConvParams& p, int width, int32_t dtype, bool step, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == GDN_B200_BF16) return launch_conv_type<__nv_bfloat16>(p, width, n, step, st);
-  if (dtype == GDN_B200_FP16) return launch_conv_type<__half>(p, width, n, step, st);
-  return launch_conv_type<float>(p, width, n, step, st);
+  if (dtype == GDN_B200_BF16) return launch_conv_type<__nv_bfloat16>(p, width, step, st);
+  if (dtype == GDN_B200_FP16) return launch_conv_type<__half>(p, width, step, st);
+  return launch_conv_type<float>(p, width, step, st);
 }
 
 int check_conv(int64_t rows, int64_t pool, int32_t channels, int32_t width, int32_t dtype,
@@ -330,8 +343,7 @@ extern "C" int gdn_b200_short_conv(const void* x, int64_t x_stride, const void* 
   p.seqs = static_cast<int>(num_seqs);
   p.channels = channels;
   p.silu = activation == GDN_B200_ACT_SILU;
-  const long long tiles = std::max<long long>(1, (total_tokens + kConvTile - 1) / kConvTile);
-  return conv_call(p, width, dtype, tiles, false, stream);
+  return conv_call(p, width, dtype, false, stream);
 }
 
 extern "C" int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const void* weight,
@@ -369,7 +381,7 @@ extern "C" int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const v
   p.slots_is64 = indices_are_int64 ? 1 : 0;
   p.channels = channels;
   p.silu = activation == GDN_B200_ACT_SILU;
-  return conv_call(p, width, dtype, batch, true, stream);
+  return conv_call(p, width, dtype, true, stream);
 }
 
 extern "C" uint64_t gdn_b200_ssm_prefill_workspace_size(int64_t num_seqs, int64_t total_tokens,

@@ -54,6 +54,37 @@ struct Pack {
   }
 };
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_bits(uint32_t x, uint32_t y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // Elements of a 16-byte vector.
 template <typename T> constexpr int kLanes = 16 / static_cast<int>(sizeof(T));
 
@@ -79,11 +110,11 @@ __device__ __forceinline__ long long slot_of(const void* idx, int is64, long lon
   return s < 0 ? -1 : s;
 }
 
-// One block reports offsets that do not rise within [0, tokens].
+// One warp reports offsets that do not rise within [0, tokens].
 __device__ __forceinline__ void check_offsets(const void* cu, int is64, int n, long long tokens,
                                               unsigned int* status) {
   bool bad = false;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
     const long long s = index_at(cu, is64, i), e = index_at(cu, is64, i + 1);
     bad |= s < 0 || e < s || e > tokens;
   }
