@@ -52,6 +52,20 @@ __device__ __forceinline__ float team_sum(float v, float* smem) {
 
 __device__ __forceinline__ float gate_act(float g, int silu) { return silu ? silu_f(g) : sigmoid_f(g); }
 
+// v[e] *= act(gate element e), two elements at a time.
+template <typename T, int V>
+__device__ __forceinline__ void apply_gate(float (&v)[V], const Pack<T, V>& gate, int silu) {
+  float g[V];
+  gate.unpack(g);
+#pragma unroll
+  for (int e = 0; e < V; e += 2) {
+    const uint64_t gp = pair(g[e], g[e + 1]);
+    const float2 y = unpair(mul2(pair(v[e], v[e + 1]), silu ? silu2(gp) : sigmoid2(gp)));
+    v[e] = y.x;
+    v[e + 1] = y.y;
+  }
+}
+
 constexpr int kNormThreads = 128;   // of a block, where a team is a warp or less
 
 template <typename T, int V, int kTeam, int kVecs>
@@ -85,12 +99,7 @@ gdn_gated_norm_kernel(const NormParams p) {
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     xv[i].unpack(xf[i]);
-    if (p.gate && !p.norm_first) {
-      float gf[V];
-      gv[i].unpack(gf);
-#pragma unroll
-      for (int e = 0; e < V; ++e) xf[i][e] *= gate_act(gf[e], p.silu);
-    }
+    if (p.gate && !p.norm_first) apply_gate<T, V>(xf[i], gv[i], p.silu);
 #pragma unroll
     for (int e = 0; e < V; ++e) ss = fmaf(xf[i][e], xf[i][e], ss);
   }
@@ -110,12 +119,7 @@ gdn_gated_norm_kernel(const NormParams p) {
 #pragma unroll
       for (int e = 0; e < V; ++e) y[e] *= wf[e];
     }
-    if (p.gate && p.norm_first) {
-      float gf[V];
-      gv[i].unpack(gf);
-#pragma unroll
-      for (int e = 0; e < V; ++e) y[e] *= gate_act(gf[e], p.silu);
-    }
+    if (p.gate && p.norm_first) apply_gate<T, V>(y, gv[i], p.silu);
     Pack<T, V> yv;
     yv.pack(y);
     yv.store(out + c);

@@ -39,44 +39,46 @@ bool wide_rows(const void* p, long long stride, int size) {
 
 // ------------------------------------------------------------ short convolution
 template <typename T, int V, int W>
-void launch_conv(const ConvParams& p, bool step, cudaStream_t st) {
-  constexpr unsigned per_block = kConvThreads / 32;
-  const unsigned grid = (p.warps + per_block - 1) / per_block;
+void launch_conv(const ConvParams& p, unsigned grid, bool step, cudaStream_t st) {
+  const size_t smem =
+      V > 1 ? 128 + static_cast<size_t>(p.tile + 2 * W - 3) * kConvThreads * V * sizeof(T) : 0;
   if (step) gdn_short_conv_step_kernel<T, V, W><<<grid, kConvThreads, 0, st>>>(p);
-  else gdn_short_conv_kernel<T, V, W><<<grid, kConvThreads, 0, st>>>(p);
+  else gdn_short_conv_kernel<T, V, W><<<grid, kConvThreads, smem, st>>>(p);
 }
 
 template <typename T, int V>
-void launch_conv_width(const ConvParams& p, int width, bool step, cudaStream_t st) {
-  if (width == 2) launch_conv<T, V, 2>(p, step, st);
-  else if (width == 3) launch_conv<T, V, 3>(p, step, st);
-  else launch_conv<T, V, 4>(p, step, st);
+void launch_conv_width(const ConvParams& p, int width, unsigned grid, bool step, cudaStream_t st) {
+  if (width == 2) launch_conv<T, V, 2>(p, grid, step, st);
+  else if (width == 3) launch_conv<T, V, 3>(p, grid, step, st);
+  else launch_conv<T, V, 4>(p, grid, step, st);
 }
 
-// Tokens of a warp: long ones re-read fewer rows before their first (W - 1 each)
+// Tokens of a block: long ones re-read fewer rows before their first (W - 1 each)
 // and load their taps less often; short ones spread a small call over the SMs.
-constexpr int kConvTileLong = 32, kConvTileShort = 8;
-constexpr long long kConvFewWarps = 148 * 32;
+// 24 KiB of rows a block (8192 tokens of 8192 channels: 48 us; 51 with 16 KiB, 53
+// with 32, 57 with 40).
+constexpr int kConvTileBytes = 24 << 10, kConvTileShort = 16;
+constexpr long long kConvFewBlocks = 148 * 6;
 
 template <typename T>
 int launch_conv_type(ConvParams& p, int width, bool step, cudaStream_t st) {
-  const int size = static_cast<int>(sizeof(T));
-  // 16-byte vectors where every row starts on one, else one channel per thread
+  // 16-byte copies of rows, four channels a thread, else one channel
+  constexpr int size = static_cast<int>(sizeof(T));
   const bool wide = p.channels % kLanes<T> == 0 && wide_rows(p.x, p.x_stride, size) &&
                     wide_rows(p.out, p.out_stride, size) && aligned(p.weight, 16) &&
                     aligned(p.bias, 16) && aligned(p.state, 16) && aligned(p.new_state, 16);
-  const int v = wide ? kLanes<T> : 1;
-  p.chan_warps = (p.channels / v + 31) / 32;
+  const int per_block = kConvThreads * (wide ? kConvVec : 1);
+  p.chan_blocks = (p.channels + per_block - 1) / per_block;
   long long n = p.tokens;   // rows of a step
   if (!step) {
-    p.tile = (p.tokens / kConvTileLong + 1) * p.chan_warps < kConvFewWarps ? kConvTileShort
-                                                                         : kConvTileLong;
+    p.tile = kConvTileBytes / (kConvThreads * kConvVec * size);
+    if ((p.tokens / p.tile + 1) * p.chan_blocks < kConvFewBlocks) p.tile = kConvTileShort;
     n = std::max<long long>(1, (p.tokens + p.tile - 1) / p.tile);
   }
-  if (n > kMaxGrid / p.chan_warps) return invalid("tokens * channels exceeds the grid limit");
-  p.warps = static_cast<unsigned>(n * p.chan_warps);
-  if (wide) launch_conv_width<T, kLanes<T>>(p, width, step, st);
-  else launch_conv_width<T, 1>(p, width, step, st);
+  if (n > kMaxGrid / p.chan_blocks) return invalid("tokens * channels exceeds the grid limit");
+  const unsigned grid = static_cast<unsigned>(n * p.chan_blocks);
+  if (wide) launch_conv_width<T, kConvVec>(p, width, grid, step, st);
+  else launch_conv_width<T, 1>(p, width, grid, step, st);
   return launched("short convolution launch");
 }
 

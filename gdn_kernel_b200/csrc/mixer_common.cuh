@@ -22,24 +22,26 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { retur
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_float(float v) { return v; }
 
-// N consecutive elements as they lie in memory: one 16-byte access, or a single
-// element where sizes or addresses allow no wider one.
+// N consecutive elements as they lie in memory: one access of 16 or 8 bytes, or a
+// single element where sizes or addresses allow no wider one.
 template <typename T, int N>
 struct Pack {
-  static constexpr bool kWide = N * sizeof(T) == 16;
-  using Raw = typename std::conditional<kWide, uint4, T>::type;
-  static_assert(kWide || N == 1, "one 16-byte vector or one element");
+  static constexpr int kBytes = N * static_cast<int>(sizeof(T));
+  using Raw = typename std::conditional<kBytes == 16, uint4,
+                                        typename std::conditional<kBytes == 8, uint2, T>::type>::type;
+  static_assert(kBytes == 16 || kBytes == 8 || N == 1, "a vector of 16 or 8 bytes, or one element");
   Raw raw;
 
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
   // Read once: no line kept in L1.
   __device__ __forceinline__ void load_stream(const T* p) {
-    if constexpr (kWide) raw = __ldcs(reinterpret_cast<const uint4*>(p));
+    if constexpr (kBytes >= 8 && N > 1) raw = __ldcs(reinterpret_cast<const Raw*>(p));
     else raw = *p;
   }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
   __device__ __forceinline__ void zero() {
-    if constexpr (kWide) raw = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (kBytes == 16) raw = make_uint4(0u, 0u, 0u, 0u);
+    else if constexpr (kBytes == 8) raw = make_uint2(0u, 0u);
     else raw = from_float<T>(0.0f);
   }
   __device__ __forceinline__ void unpack(float (&f)[N]) const {
@@ -85,12 +87,41 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+// sigmoid(v) = 1 / (1 + 2^(-v log2 e)) and v sigmoid(v), two at a time: one
+// reciprocal of both denominators' product serves the two, which takes a quarter
+// of the special-function operations off the path that bounds an activation.
+// The exponent stops at 62 so that the product stays finite, and the 2^-62 that
+// sigmoid stops at is taken off, exactly, so that a closed gate is 0 (where sigmoid
+// is small but not yet 0, that is an error of 2^-62).  A NaN reaches only its own
+// result, through silu.
+__device__ __forceinline__ float fast_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t v) {
+  constexpr float kMinusLog2e = -1.4426950408889634f;
+  const float2 t = unpair(mul2(v, pair(kMinusLog2e, kMinusLog2e)));
+  const uint64_t d = add2(pair(fast_exp2(fminf(t.x, 62.0f)), fast_exp2(fminf(t.y, 62.0f))),
+                          pair(1.0f, 1.0f));
+  const float2 f = unpair(d);
+  const float r = fast_rcp(f.x * f.y);
+  constexpr float kFloor = -2.168404344971009e-19f;   // -2^-62
+  return fma2(pair(f.y, f.x), pair(r, r), pair(kFloor, kFloor));
+}
+__device__ __forceinline__ uint64_t silu2(uint64_t v) { return mul2(v, sigmoid2(v)); }
+__device__ __forceinline__ float sigmoid_f(float v) {
+  return v != v ? v : fast_rcp(1.0f + fast_exp2(-1.4426950408889634f * v));
+}
+__device__ __forceinline__ float silu_f(float v) { return unpair(silu2(pair(v, 0.0f))).x; }
+
 // Elements of a 16-byte vector.
 template <typename T> constexpr int kLanes = 16 / static_cast<int>(sizeof(T));
-
-// v sigmoid(v) and sigmoid(v); exp(-v) = inf gives 0 as it should.
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
-__device__ __forceinline__ float silu_f(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 
 __device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
   return is64 ? reinterpret_cast<const long long*>(p)[i]

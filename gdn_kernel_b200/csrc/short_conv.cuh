@@ -4,17 +4,18 @@
 // tokens.  The new carried state is the last W-1 rows of u.
 //
 // Both forms move each element once and do 2 W + 5 operations on it, so memory
-// bounds them.  A thread owns one 16-byte vector of channels (one channel where
-// sizes or addresses are not 16-byte multiples); its taps stay in fp32
-// registers and sums are fp32, rounded once at the end.
+// bounds them.  A thread owns four channels (one where sizes or addresses do not
+// allow 16-byte copies); its taps stay in fp32 registers and sums are fp32,
+// rounded once at the end.
 #pragma once
 
+#include "gdn_ptx.cuh"
 #include "mixer_common.cuh"
 
 namespace gdn {
 
 constexpr int kConvThreads = 128;
-constexpr int kConvBatch = 4;    // rows loaded while the four before them are worked on
+constexpr int kConvVec = 4;      // channels of a thread
 
 struct ConvParams {
   const void* x;               // [T, D], rows x_stride apart
@@ -29,9 +30,8 @@ struct ConvParams {
   unsigned int* status;
   long long x_stride, out_stride, pool, tokens;
   int cu_is64, slots_is64, seqs, channels, silu;
-  int tile;                    // tokens of a warp (prompts)
-  unsigned int chan_warps;     // warps over the channels; all warps are those times tiles or rows
-  unsigned int warps;
+  int tile;                    // prompts: tokens of a block
+  unsigned int chan_blocks;    // blocks over the channels; the grid is those times tiles or rows
 };
 
 // The taps of V channels, two channels to a pair where V allows it.
@@ -94,9 +94,9 @@ struct ConvWindow {
 #pragma unroll
       for (int k = 0; k < W - 1; ++k) s = fma2(taps.w[k][i], u[k][i], s);
       s = fma2(taps.w[W - 1][i], cur[i], s);
-      const float2 f = unpair(s);
-      y[2 * i] = silu ? silu_f(f.x) : f.x;
-      if constexpr (V > 1) y[2 * i + 1] = silu ? silu_f(f.y) : f.y;
+      const float2 f = unpair(silu ? silu2(s) : s);
+      y[2 * i] = f.x;
+      if constexpr (V > 1) y[2 * i + 1] = f.y;
 #pragma unroll
       for (int k = 0; k + 1 < W - 1; ++k) u[k][i] = u[k + 1][i];
       u[W - 2][i] = cur[i];
@@ -107,26 +107,72 @@ struct ConvWindow {
   }
 };
 
-// Prompts: a warp takes p.tile consecutive packed tokens of 32 V channels and
-// walks the sequences that touch them.  The thread that holds a
+// Prompts: a block takes p.tile consecutive packed tokens of kConvThreads V
+// channels and walks the sequences that touch them.  The thread that holds a
 // sequence's first token also writes its new state, after it has read the old
 // one, so that the two may be the same memory.
+//
+// V = kConvVec: all the block's rows (and the W - 1 before them) come to shared
+// memory as bulk copies that start before the sequences are looked up.  With the
+// rows in registers instead, four loaded ahead, the copies in flight were too few
+// (8192 tokens of 8192 channels: 63 us).  V = 1: plain loads.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const ConvParams p) {
-  const unsigned int id = blockIdx.x * (kConvThreads / 32) + threadIdx.x / 32;
-  if (id >= p.warps) return;
-  const int d = static_cast<int>(id % p.chan_warps * 32 + threadIdx.x % 32) * V;
-  const long long t0 = static_cast<long long>(id / p.chan_warps) * p.tile;
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr bool kStaged = V == kConvVec;
+  constexpr int kRow = kConvThreads * V;          // elements of a staged row
+  const int c0 = static_cast<int>(blockIdx.x % p.chan_blocks) * kRow;
+  const int d = c0 + static_cast<int>(threadIdx.x) * V;
+  const long long t0 = static_cast<long long>(blockIdx.x / p.chan_blocks) * p.tile;
   const long long t1 = min(t0 + p.tile, p.tokens);
   const bool last_tile = t1 == p.tokens;
+  const long long r0 = max(t0 - (W - 1), 0LL);    // rows staged: [r0, r1)
+  const long long r1 = min(t1 + W - 2, p.tokens);
+  const T* rows = reinterpret_cast<const T*>(smem + 128) + threadIdx.x * V;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem);
+  if constexpr (kStaged) {
+    if (threadIdx.x == 0) {
+      mbar_init(bar, 1);
+      fence_mbarrier_init();
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int n = static_cast<int>(r1 - r0);
+      const uint32_t bytes = static_cast<uint32_t>(min(kRow, p.channels - c0) * sizeof(T));
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, n * bytes);
+      __syncwarp();
+      for (int i = threadIdx.x; i < n; i += 32)
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+            ::"r"(smem_u32(smem + 128 + static_cast<size_t>(i) * kRow * sizeof(T))),
+            "l"(static_cast<const T*>(p.x) + (r0 + i) * p.x_stride + c0), "r"(bytes),
+            "r"(smem_u32(bar))
+            : "memory");
+    }
+  }
   int i = count_below(p.cu, p.cu_is64, p.seqs, t0);
-  if (id == 0) check_offsets(p.cu, p.cu_is64, p.seqs, p.tokens, p.status);
-  if (d >= p.channels) return;
+  if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.cu, p.cu_is64, p.seqs, p.tokens, p.status);
+  const bool live = d < p.channels;
   const bool reporter = d == 0;
   const T* x = static_cast<const T*>(p.x) + d;
   T* out = static_cast<T*>(p.out) + d;
   ConvTaps<T, V, W> taps;
-  taps.load(p, d);
+  if (live) taps.load(p, d);
+  if constexpr (kStaged) {
+    // (a second wait in case the first ran out: no copy may outlive the block)
+    if (!mbar_wait(bar, 0)) {
+      if (threadIdx.x == 0) atomicOr(p.status, kStatusTmaTimeout);
+      mbar_wait(bar, 0);
+      return;
+    }
+  }
+  if (!live) return;
+  auto row_at = [&](long long t) {
+    Pack<T, V> v;
+    if constexpr (kStaged) v.load(rows + static_cast<int>(t - r0) * kRow);
+    else v.load(x + t * p.x_stride);
+    return v;
+  };
 
   // the sequence that is running at t0, then those that start in this tile
   for (i = max(i - 1, 0); i < p.seqs; ++i) {
@@ -162,43 +208,26 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) {
           const long long pos = len - (W - 1) + k;   // row k holds this position of the tokens
-          Pack<T, V> v;
-          v.zero();
-          if (pos >= 0) v.load(x + (s + pos) * p.x_stride);
+          T* to = ns + static_cast<long long>(k) * p.channels;
+          if (pos >= 0) {
+            Pack<T, V> v;
+            v.load(x + (s + pos) * p.x_stride);
+            v.store(to);
+          }
 #pragma unroll
-          for (int j = 0; j < W - 1; ++j)
-            if (pos < 0 && j == W - 1 + pos) v = old[j];
-          v.store(ns + static_cast<long long>(k) * p.channels);
+          for (int j = k; j < W - 1; ++j)   // an old row, in a sequence shorter than the window
+            if (pos + W - 1 == j) old[j].store(to);
         }
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < W - 1; ++k) {
-        Pack<T, V> v;
-        v.load(x + (a - (W - 1) + k) * p.x_stride);
-        win.set(k, v);
-      }
+      for (int k = 0; k < W - 1; ++k) win.set(k, row_at(a - (W - 1) + k));
     }
-
-    const T* src = x + a * p.x_stride;
     T* dst = out + a * p.out_stride;
-    int left = static_cast<int>(z - a);
-    Pack<T, V> next[kConvBatch];
-#pragma unroll
-    for (int j = 0; j < kConvBatch; ++j)
-      if (j < left) next[j].load_stream(src + j * p.x_stride);
-    for (; left > 0; left -= kConvBatch) {
-      Pack<T, V> in[kConvBatch];
-      src += kConvBatch * p.x_stride;
-#pragma unroll
-      for (int j = 0; j < kConvBatch; ++j) {
-        in[j] = next[j];
-        if (j + kConvBatch < left) next[j].load_stream(src + j * p.x_stride);
-      }
-#pragma unroll
-      for (int j = 0; j < kConvBatch; ++j)
-        if (j < left) win.row(taps, in[j], p.silu).store(dst + j * p.out_stride);
-      dst += kConvBatch * p.out_stride;
+#pragma unroll 8
+    for (long long t = a; t < z; ++t) {
+      win.row(taps, row_at(t), p.silu).store(dst);
+      dst += p.out_stride;
     }
   }
 }
@@ -206,11 +235,9 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
 // Single tokens: one row per batch entry, its window in the pool.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_step_kernel(const ConvParams p) {
-  const unsigned int id = blockIdx.x * (kConvThreads / 32) + threadIdx.x / 32;
-  if (id >= p.warps) return;
-  const int d = static_cast<int>(id % p.chan_warps * 32 + threadIdx.x % 32) * V;
+  const int d = static_cast<int>(blockIdx.x % p.chan_blocks * kConvThreads + threadIdx.x) * V;
   if (d >= p.channels) return;
-  const long long b = id / p.chan_warps;
+  const long long b = blockIdx.x / p.chan_blocks;
   const long long slot = slot_of(p.slots, p.slots_is64, b, p.pool, p.status, d == 0);
   T* out = static_cast<T*>(p.out) + b * p.out_stride + d;
   if (slot < 0) {
