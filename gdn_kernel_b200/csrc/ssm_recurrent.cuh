@@ -44,19 +44,40 @@ __device__ __forceinline__ float ssm_step_size(float v) {
   return v > 20.0f ? v : log1pf(expf(v));
 }
 
+// A token's operands of one thread, as they lie in memory: eight lanes' columns
+// of B and C, and the thread's rows of x.
 template <int N>
-__device__ __forceinline__ void load_columns(const __nv_bfloat16* p, int l8, float (&f)[N / 8]) {
+struct SsmToken {
+  uint2 b[N / 32], c[N / 32];
+  __nv_bfloat16 x[kSsmRows], dt;
+  __device__ __forceinline__ void load(const SsmParams& p, long long t, int head, int group, int l8,
+                                       int row0) {
+    const __nv_bfloat16* B = p.B + t * p.b_stride + group * N + 4 * l8;
+    const __nv_bfloat16* C = p.C + t * p.c_stride + group * N + 4 * l8;
+#pragma unroll
+    for (int j = 0; j < N / 32; ++j) {
+      b[j] = *reinterpret_cast<const uint2*>(B + 32 * j);
+      c[j] = *reinterpret_cast<const uint2*>(C + 32 * j);
+    }
+    const __nv_bfloat16* src = p.x + t * p.x_stride + head * p.head_dim + row0;
+#pragma unroll
+    for (int i = 0; i < kSsmRows; ++i) x[i] = src[kSsmThreads / 8 * i];
+    dt = p.dt[t * p.dt_stride + head];
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void unpack_columns(const uint2 (&u)[N / 32], float (&f)[N / 8]) {
 #pragma unroll
   for (int j = 0; j < N / 32; ++j) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p + 4 * l8 + 32 * j);
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[j].x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[j].y));
     f[4 * j] = a.x; f[4 * j + 1] = a.y; f[4 * j + 2] = b.x; f[4 * j + 3] = b.y;
   }
 }
 
-// kPrompt: the tokens of sequence blockIdx.y in order; else the one token of
-// batch entry blockIdx.y.
+// kPrompt: the tokens of sequence blockIdx.y in order, the next one's operands
+// loaded while one is worked on; else the one token of batch entry blockIdx.y.
 template <int N, bool kPrompt>
 __global__ void __launch_bounds__(kSsmThreads) gdn_ssm_recurrent_kernel(const SsmParams p) {
   const int P = p.head_dim;
@@ -89,6 +110,8 @@ __global__ void __launch_bounds__(kSsmThreads) gdn_ssm_recurrent_kernel(const Ss
     return;
   }
 
+  SsmToken<N> tok;
+  if (t < end) tok.load(p, t, head, group, l8, row0);
   float h[kSsmRows][N / 8];
   const bool carried = p.state && slot >= 0 && (!p.has_state || p.has_state[seq]);
 #pragma unroll
@@ -106,15 +129,16 @@ __global__ void __launch_bounds__(kSsmThreads) gdn_ssm_recurrent_kernel(const Ss
   const float bias = p.dt_bias ? p.dt_bias[head] : 0.0f;
   const float D = p.D ? p.D[head] : 0.0f;
   for (; t < end; ++t) {
-    const float step = ssm_step_size(to_float(p.dt[t * p.dt_stride + head]) + bias);
+    const SsmToken<N> now = tok;
+    if (kPrompt && t + 1 < end) tok.load(p, t + 1, head, group, l8, row0);
+    const float step = ssm_step_size(to_float(now.dt) + bias);
     const float decay = expf(A * step);
     float Bf[N / 8], Cf[N / 8];
-    load_columns<N>(p.B + t * p.b_stride + group * N, l8, Bf);
-    load_columns<N>(p.C + t * p.c_stride + group * N, l8, Cf);
+    unpack_columns<N>(now.b, Bf);
+    unpack_columns<N>(now.c, Cf);
 #pragma unroll
     for (int i = 0; i < kSsmRows; ++i) {
-      const int row = row0 + kStep * i;
-      const float x = to_float(p.x[t * p.x_stride + head * P + row]);
+      const float x = to_float(now.x[i]);
       const float xs = x * step;
       float y = 0.0f;
 #pragma unroll
@@ -125,7 +149,8 @@ __global__ void __launch_bounds__(kSsmThreads) gdn_ssm_recurrent_kernel(const Ss
       y += __shfl_xor_sync(0xffffffffu, y, 1);
       y += __shfl_xor_sync(0xffffffffu, y, 2);
       y += __shfl_xor_sync(0xffffffffu, y, 4);
-      if (l8 == 0) p.out[(t * p.heads + head) * P + row] = __float2bfloat16_rn(fmaf(D, x, y));
+      if (l8 == 0)
+        p.out[(t * p.heads + head) * P + row0 + kStep * i] = __float2bfloat16_rn(fmaf(D, x, y));
     }
   }
   if (wslot < 0) return;

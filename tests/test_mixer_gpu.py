@@ -207,6 +207,13 @@ def test_scan_lengths(P, N, lens):
     run_scan(lens, 4, P, 2, N)
 
 
+@pytest.mark.parametrize("P,N", [(64, 128), (128, 64)])
+@pytest.mark.parametrize("lens", [[0, 0], [10], [11], [3, 0, 17, 1, 9], [2] * 40, [40] + [0] * 7])
+def test_scan_short_sequences(P, N, lens):
+    """Around the length below which prompts run token by token."""
+    run_scan(lens, 2, P, 2, N, seed=14)
+
+
 @pytest.mark.parametrize("H,G", [(1, 1), (3, 1), (5, 5), (6, 2), (24, 8)])
 def test_scan_head_layouts(H, G):
     run_scan([90, 200], H, 64, G, 128, seed=3)
