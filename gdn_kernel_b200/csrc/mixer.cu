@@ -303,9 +303,20 @@ int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, void* wor
     else
       gdn_ssm_piece_state_kernel<128><<<pieces, kStateThreads, kStateSmem, st>>>(tx, tb, sp);
   }
-  const dim3 grid(units, static_cast<unsigned>(plan.max_full + seqs));
-  if (state_dim == 64) gdn_ssm_scan_kernel<64><<<grid, kScanThreads, kScanSmem, st>>>(tx, tb, tc, sp);
-  else gdn_ssm_scan_kernel<128><<<grid, kScanThreads, kScanSmem, st>>>(tx, tb, tc, sp);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(units, static_cast<unsigned>(plan.max_full + seqs));
+  cfg.blockDim = dim3(kScanThreads);
+  cfg.dynamicSmemBytes = kScanSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute beside[1];
+  beside[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  beside[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = beside;
+  cfg.numAttrs = plan.max_full > 0 ? 1 : 0;   // after the kernel of the pieces only
+  const cudaError_t e =
+      state_dim == 64 ? cudaLaunchKernelEx(&cfg, gdn_ssm_scan_kernel<64>, tx, tb, tc, sp)
+                      : cudaLaunchKernelEx(&cfg, gdn_ssm_scan_kernel<128>, tx, tb, tc, sp);
+  if (e != cudaSuccess) return lib_cuda_fail(e, "selective scan launch");
   return launched("selective scan launch");
 }
 

@@ -413,6 +413,8 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
   // Chunk i of the order, from the end: false once the decays leave nothing of it.
   auto more = [&](int i) { return later[2 * (i & 1)] > kScanGone; };
 
+  // the scan's blocks may take the SMs that this grid leaves or has done with
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (nch == 0) {
     // no such piece, or a sequence's last
   } else if (warp == 0) {
@@ -817,11 +819,15 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 #pragma unroll
       for (int j = 0; j < kScanCols / 2; ++j) {
         const float* s = src + 2 * j * N + row;
-        h[j] = fma2(pair(__ldg(s), __ldg(s + N)), f2, h[j]);
+        h[j] = fma2(pair(__ldcg(s), __ldcg(s + N)), f2, h[j]);
       }
     };
     bool carried;
     const long long slot = find_state(carried);
+    // The kernel before made the states of pieces; this one may have started
+    // beside it (programmatic launch), and only here needs it to be done.
+    if (it.pieces > 1 && (it.piece > 0 || p.state == p.new_state))
+      asm volatile("griddepcontrol.wait;" ::: "memory");
     if (state_row) {   // the start: what the pieces before this one leave, and the carried state
       float log_decay = 0.0f;
       const long long row0 = static_cast<long long>(it.first_row) * sp.parts;
@@ -835,7 +841,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                     : p.state + slot * per_slot + hbase;
         add_state(src, log_decay);
         if (r >= 0)
-          log_decay += sp.seg_decay[(row0 + r) * p.heads + head];
+          log_decay += __ldcg(sp.seg_decay + (row0 + r) * p.heads + head);
       }
     }
     bool ok = true;
