@@ -6,7 +6,9 @@
 //   r' = r + s u,  u = x or rms(x) w_b;      y = rms(r') (w + offset)
 // with rms(v) = v / sqrt(mean(v^2) + eps) over the group.
 //
-// Memory bounds both: each element is read once, kept in registers between the
+// Memory bounds both (8192 rows of 32 groups of 128: 37 us, 5.4 TB/s; 8192 rows of
+// 2048 with an fp32 residual and both norms: 35 us, 5.7 TB/s; a plain copy reaches
+// 6.5): each element is read once, kept in registers between the
 // sum of squares and the scaling, and written once.  Sums are fp32.  `kTeam`
 // threads share a group (part of a warp, a warp, or a block), each holding
 // kVecs 16-byte vectors of every operand.  Rows that no such shape fits (sizes

@@ -15,7 +15,7 @@
 //   Yo = C h           128 x 64 x N, h rounded to bf16
 //   Yd = M X           128 x 64 x 128, M rounded to bf16 in tensor memory
 // Yo and Yd stay apart because their row factors differ; the output rounds once
-// more.  The roundings of h and M are 2^-9 of their terms each at most, as in
+// more.  The roundings of h and M are 2^-8 of their terms each at most, as in
 // the bf16 output itself.
 //
 // Decays come from sums towards the chunk's end, sfx_t = L_Q - L_t, which are
@@ -36,6 +36,15 @@
 // made while dS and Yo run.
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
 // there, so nothing of them (not even a NaN) enters a product's sum.
+//
+// Measured: 8192 tokens, 64 heads of 64, state 128, 99 us with the kernel of the
+// pieces' states (20 us); 20011 ragged tokens of 32 heads of 128, state 64, 173 us.
+// A chunk takes about 4000 clocks, its shared-memory traffic 3070 (384 KB: 208 of
+// product operands, 80 of arriving tiles, 96 of x, w X and h), the tensor pipe is
+// active for 2750; the rest is handing over.  128 tokens a chunk, because products
+// of 64 rows run at half rate; 64 columns, because 128 need 320 KB of shared memory.
+// The roles' loops together have to stay near 32 KB of code: at 75 KB a chunk took
+// 7600 clocks, waiting for instructions.
 #pragma once
 
 #include <cuda.h>
