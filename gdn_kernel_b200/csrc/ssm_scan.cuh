@@ -26,12 +26,12 @@
 // so e^{L_t - L_s} step_s is a row factor times a column factor.
 //
 // Twenty-eight warps with one role each, handing over through mbarriers:
-//   0-1 gates                              2 TMA, two stages of {C, B, X}
-//   3 issues the products                  4-7, 24-27 S -> M (thread = token row)
+//   0 issues the products                  3 TMA, two stages of {C, B, X}
+//   1-2 gates                              4-7, 24-27 S -> M (thread = token row)
 //   8-11 the state in registers (thread = state row)
 //   12-15 outputs (thread = token row)     16-23 w X (thread = half a token row)
 // One warp of each four works on a quarter of the rows, and M's last rows are the
-// longest: the gates sit with the first two quarters.
+// longest: the warp that issues sits with the first quarter.
 // The products of a chunk are issued as dS, Yo, S of the next chunk, Yd: M is then
 // made while dS and Yo run.
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
@@ -631,7 +631,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     }
   } else if (warp < 4) {
     scan_set_regs<kRegsIssue>();
-    if (warp == 2) {
+    if (warp == 3) {
       // ---------------------------------------------- TMA
       int issued = 0;
       bool ok = true;
@@ -660,7 +660,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
           mbar_wait(bars + kBFullX + (c & 1), (c >> 1) & 1);
           mbar_wait(bars + kBFullBC + (c & 1), (c >> 1) & 1);
         }
-    } else if (warp == 3) {
+    } else if (warp == 0) {
       // ---------------------------------------------- products
       // Every lane runs the whole sequence and an elected one issues: the warp
       // never diverges, so descriptors stay in uniform registers.  (Inside a
@@ -731,9 +731,9 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       // Two warps take turns; a chunk's dt are on their way while the chunk
       // before it (of this warp) is worked on.
       ScanGates gates;
-      gates.start(p, t_begin, len, head, warp);
+      gates.start(p, t_begin, len, head, warp - 1);
 #pragma unroll 1
-      for (int c = warp; c < nch; c += 2) {
+      for (int c = warp - 1; c < nch; c += 2) {
         const int st = c & 1;
         gates.make(c, c + 2);
         if (c >= 2 && !wait(kBGateEmpty + st, (c >> 1) - 1, kStatusMmaTimeout)) break;
