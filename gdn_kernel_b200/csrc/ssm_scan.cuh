@@ -986,6 +986,7 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   __syncthreads();
   tc_fence_after();
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, static_cast<unsigned int>(*abort_flag));
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // this grid ends after the one before it
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 

@@ -474,17 +474,40 @@ def test_calls_follow_the_current_stream():
     assert torch.equal(ref, want)
 
 
-def test_calls_are_captured_in_a_graph():
-    ins = scan_inputs(200, 4, 64, 1, 128)
-    cu = offsets([150, 50])
-    out, ns = torch.empty(200, 4, 64, dtype=BF).cuda(), torch.empty(2, 4, 64, 128).cuda()
-    ws = torch.empty(max(1, M.ssm_prefill_workspace_bytes(2, 200, 4, 64, 128)), dtype=torch.uint8,
-                     device="cuda")
+@pytest.mark.parametrize("lens", [[150, 50], [1450, 50]])
+def test_calls_are_captured_in_a_graph(lens):
+    T = sum(lens)
+    ins = scan_inputs(T, 4, 64, 1, 128)
+    cu = offsets(lens)
+    out, ns = torch.empty(T, 4, 64, dtype=BF).cuda(), torch.empty(2, 4, 64, 128).cuda()
+    need = M.ssm_prefill_workspace_bytes(2, T, 4, 64, 128)
+    assert (need > 0) == (T > 1000)              # the longer one runs in pieces
+    ws = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
     M.gdn_ssm_prefill(*ins, None, cu, out, ns, workspace=ws)
     want, ws_want = out.clone(), ns.clone()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         M.gdn_ssm_prefill(*ins, None, cu, out, ns, workspace=ws)
-    out.zero_(), ns.zero_()
-    g.replay()
-    assert torch.equal(out, want) and torch.equal(ns, ws_want)
+    for _ in range(3):
+        out.zero_(), ns.zero_(), ws.zero_()
+        g.replay()
+        g.replay()
+        assert torch.equal(out, want) and torch.equal(ns, ws_want)
+
+
+def test_calls_on_two_streams_with_workspaces_of_their_own():
+    a = [scan_inputs(T, 8, 64, 2, 128, seed=T) for T in (3000, 2500)]
+    cu = [offsets([3000]), offsets([2000, 500])]
+    want = [M.ssm_prefill(*i, None, c) for i, c in zip(a, cu)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(M.ssm_prefill(*a[k], None, cu[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for out, ns in got[k]:
+            assert torch.equal(out, want[k][0]) and torch.equal(ns, want[k][1])
+    status_clean()
