@@ -75,8 +75,11 @@ int launch_conv_type(ConvParams& p, int width, bool step, cudaStream_t st) {
     if ((p.tokens / p.tile + 1) * p.chan_blocks < kConvFewBlocks) p.tile = kConvTileShort;
     n = std::max<long long>(1, (p.tokens + p.tile - 1) / p.tile);
   }
-  if (n > kMaxGrid / p.chan_blocks) return invalid("tokens * channels exceeds the grid limit");
-  const unsigned grid = static_cast<unsigned>(n * p.chan_blocks);
+  const long long blocks = step ? n : n + p.seqs;
+  if (blocks > kMaxGrid / p.chan_blocks) return invalid("tokens * channels exceeds the grid limit");
+  const unsigned grid = static_cast<unsigned>(blocks * p.chan_blocks);
+  p.tile_blocks = static_cast<unsigned>(n * p.chan_blocks);
+  p.lookup_first = p.tokens <= 2LL * kConvShort * p.seqs;
   if (wide) launch_conv_width<T, kConvVec>(p, width, grid, step, st);
   else launch_conv_width<T, 1>(p, width, grid, step, st);
   return launched("short convolution launch");
@@ -336,6 +339,7 @@ extern "C" int gdn_b200_short_conv(const void* x, int64_t x_stride, const void* 
   lib_clear_error();
   if (int rc = check_conv(total_tokens, pool_size, channels, width, dtype, activation)) return rc;
   if (num_seqs < 0 || num_seqs > kMaxGrid) return invalid("num_seqs must be in [0, 2^31)");
+  if (total_tokens > (1LL << 30)) return invalid("total_tokens exceeds 2^30");
   if (num_seqs == 0) return GDN_B200_OK;
   if (!weight || !cu_seqlens || !new_state || (total_tokens > 0 && (!x || !output)))
     return invalid("null pointer argument");

@@ -16,6 +16,7 @@ namespace gdn {
 
 constexpr int kConvThreads = 128;
 constexpr int kConvVec = 4;      // channels of a thread
+constexpr int kConvShort = 16;   // tokens up to which a sequence has blocks of its own
 
 struct ConvParams {
   const void* x;               // [T, D], rows x_stride apart
@@ -32,6 +33,8 @@ struct ConvParams {
   int cu_is64, slots_is64, seqs, channels, silu;
   int tile;                    // prompts: tokens of a block
   unsigned int chan_blocks;    // blocks over the channels; the grid is those times tiles or rows
+  unsigned int tile_blocks;    // prompts: blocks of tiles; those of short sequences follow
+  int lookup_first;            // prompts: look for a tile's sequences before its rows are loaded
 };
 
 // The taps of V channels, two channels to a pair where V allows it.
@@ -107,10 +110,52 @@ struct ConvWindow {
   }
 };
 
+// A whole sequence of a few tokens by each thread: old rows, tokens, new rows.
+template <typename T, int V, int W>
+__device__ __forceinline__ void short_sequence(const ConvParams& p, int seq, int d) {
+  const long long s = index_at(p.cu, p.cu_is64, seq);
+  const long long e = index_at(p.cu, p.cu_is64, seq + 1);
+  if (s < 0 || e < s || e > p.tokens || e - s > kConvShort) return;   // tiles do and report those
+  const long long slot = slot_of(p.slots, p.slots_is64, seq, p.pool, p.status, d == 0);
+  const bool carried = p.state && slot >= 0 && (!p.has_state || p.has_state[seq]);
+  if (d >= p.channels) return;
+  const int len = static_cast<int>(e - s);
+  const T* x = static_cast<const T*>(p.x) + s * p.x_stride + d;
+  T* out = static_cast<T*>(p.out) + s * p.out_stride + d;
+  Pack<T, V> hist[W - 1];     // the last W - 1 rows so far
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) {
+    hist[k].zero();
+    if (carried)
+      hist[k].load(static_cast<const T*>(p.state) + (slot * (W - 1) + k) * p.channels + d);
+  }
+  Pack<T, V> next;
+  if (len > 0) next.load_stream(x);
+  ConvTaps<T, V, W> taps;
+  taps.load(p, d);
+  ConvWindow<T, V, W> win;
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) win.set(k, hist[k]);
+  for (int t = 0; t < len; ++t) {
+    const Pack<T, V> in = next;
+    if (t + 1 < len) next.load_stream(x + (t + 1) * p.x_stride);
+    win.row(taps, in, p.silu).store(out + t * p.out_stride);
+#pragma unroll
+    for (int k = 0; k + 1 < W - 1; ++k) hist[k] = hist[k + 1];
+    hist[W - 2] = in;
+  }
+  if (slot < 0) return;
+  T* ns = static_cast<T*>(p.new_state) + slot * (W - 1) * p.channels + d;
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) hist[k].store(ns + static_cast<long long>(k) * p.channels);
+}
+
 // Prompts: a block takes p.tile consecutive packed tokens of kConvThreads V
-// channels and walks the sequences that touch them.  The thread that holds a
-// sequence's first token also writes its new state, after it has read the old
-// one, so that the two may be the same memory.
+// channels and walks the sequences of more than kConvShort tokens that touch them.
+// The thread that holds a sequence's first token also writes its new state, after
+// it has read the old one, so that the two may be the same memory.  Shorter
+// sequences have blocks of their own: a tile would work through many of them one
+// after the other (64 of one token, 8192 channels: 21 us).
 //
 // V = kConvVec: all the block's rows (and the W - 1 before them) come to shared
 // memory as bulk copies that start before the sequences are looked up.  With the
@@ -123,13 +168,52 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
   constexpr int kRow = kConvThreads * V;          // elements of a staged row
   const int c0 = static_cast<int>(blockIdx.x % p.chan_blocks) * kRow;
   const int d = c0 + static_cast<int>(threadIdx.x) * V;
-  const long long t0 = static_cast<long long>(blockIdx.x / p.chan_blocks) * p.tile;
-  const long long t1 = min(t0 + p.tile, p.tokens);
-  const bool last_tile = t1 == p.tokens;
-  const long long r0 = max(t0 - (W - 1), 0LL);    // rows staged: [r0, r1)
-  const long long r1 = min(t1 + W - 2, p.tokens);
+  if (blockIdx.x >= p.tile_blocks) {
+    short_sequence<T, V, W>(p, static_cast<int>((blockIdx.x - p.tile_blocks) / p.chan_blocks), d);
+    return;
+  }
+  // (tokens are below 2^30, so that tile ends are ints too)
+  const int tokens = static_cast<int>(p.tokens);
+  const int t0 = static_cast<int>(blockIdx.x / p.chan_blocks) * p.tile;
+  const int t1 = min(t0 + p.tile, tokens);
+  const int r0 = max(t0 - (W - 1), 0);            // rows staged: [r0, r1)
+  const int r1 = min(t1 + W - 2, tokens);
   const T* rows = reinterpret_cast<const T*>(smem + 128) + threadIdx.x * V;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem);
+  // The sequences of the tile that are done here, 32 looked at together, a lane
+  // each: work(sequence, its bounds) by whole warps.
+  const int lane = threadIdx.x & 31;
+  int first = 0;
+  auto find_first = [&] { first = max(count_below(p.cu, p.cu_is64, p.seqs, t0) - 1, 0); };
+  auto for_each = [&](auto work) {
+    for (int base = first; base < p.seqs; base += 32) {
+      int s = 0, e = 0;
+      bool past = true;
+      if (base + lane < p.seqs) {
+        const long long from = index_at(p.cu, p.cu_is64, base + lane);
+        const long long to = index_at(p.cu, p.cu_is64, base + lane + 1);
+        past = from >= t1;
+        if (from >= 0 && to <= tokens && to - from > kConvShort) {
+          s = static_cast<int>(from);
+          e = static_cast<int>(to);
+        }
+      }
+      unsigned int todo = __ballot_sync(0xffffffffu, !past && e > t0);
+      while (todo) {
+        const int k = __ffs(todo) - 1;
+        todo &= todo - 1;
+        work(base + k, __shfl_sync(0xffffffffu, s, k), __shfl_sync(0xffffffffu, e, k));
+      }
+      if (__any_sync(0xffffffffu, past)) return;
+    }
+  };
+  if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.cu, p.cu_is64, p.seqs, p.tokens, p.status);
+  if (p.lookup_first) {   // most sequences are short: nothing to load for many tiles
+    bool any = false;
+    find_first();
+    for_each([&](int, int, int) { any = true; });
+    if (!any) return;
+  }
   if constexpr (kStaged) {
     if (threadIdx.x == 0) {
       mbar_init(bar, 1);
@@ -137,7 +221,7 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-      const int n = static_cast<int>(r1 - r0);
+      const int n = r1 - r0;
       const uint32_t bytes = static_cast<uint32_t>(min(kRow, p.channels - c0) * sizeof(T));
       if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, n * bytes);
       __syncwarp();
@@ -145,78 +229,59 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
         asm volatile(
             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
             ::"r"(smem_u32(smem + 128 + static_cast<size_t>(i) * kRow * sizeof(T))),
-            "l"(static_cast<const T*>(p.x) + (r0 + i) * p.x_stride + c0), "r"(bytes),
+            "l"(static_cast<const T*>(p.x) + static_cast<long long>(r0 + i) * p.x_stride + c0), "r"(bytes),
             "r"(smem_u32(bar))
             : "memory");
     }
   }
-  int i = count_below(p.cu, p.cu_is64, p.seqs, t0);
-  if (blockIdx.x == 0 && threadIdx.x < 32) check_offsets(p.cu, p.cu_is64, p.seqs, p.tokens, p.status);
+  if (!p.lookup_first) find_first();   // while the rows are on their way
   const bool live = d < p.channels;
-  const bool reporter = d == 0;
   const T* x = static_cast<const T*>(p.x) + d;
   T* out = static_cast<T*>(p.out) + d;
   ConvTaps<T, V, W> taps;
   if (live) taps.load(p, d);
   if constexpr (kStaged) {
-    // (a second wait in case the first ran out: no copy may outlive the block)
-    if (!mbar_wait(bar, 0)) {
+    if (!__syncthreads_and(mbar_wait(bar, 0))) {
       if (threadIdx.x == 0) atomicOr(p.status, kStatusTmaTimeout);
-      mbar_wait(bar, 0);
+      mbar_wait(bar, 0);   // no copy may outlive the block
       return;
     }
   }
-  if (!live) return;
-  auto row_at = [&](long long t) {
+  auto row_at = [&](int t) {
     Pack<T, V> v;
-    if constexpr (kStaged) v.load(rows + static_cast<int>(t - r0) * kRow);
+    if constexpr (kStaged) v.load(rows + (t - r0) * kRow);
     else v.load(x + t * p.x_stride);
     return v;
   };
 
-  // the sequence that is running at t0, then those that start in this tile
-  for (i = max(i - 1, 0); i < p.seqs; ++i) {
-    const long long s = index_at(p.cu, p.cu_is64, i);
-    const long long e = index_at(p.cu, p.cu_is64, i + 1);
-    if (s >= t1 && !(last_tile && s == p.tokens)) break;
-    if (s < 0 || e < s || e > p.tokens) {
-      if (reporter) atomicOr(p.status, kMixerBadSeqlens);
-      continue;
-    }
+  for_each([&](int i, int s, int e) {
+    if (!live) return;
     // A sequence's first W - 1 tokens, which read the old state, belong to the
     // tile of its start even where they reach past it.
     const bool starts = s >= t0;
-    const long long a = starts ? s : max(t0, s + W - 1);   // the tokens done here: [a, z)
-    const long long z = starts ? min(e, max(t1, s + W - 1)) : min(e, t1);
-    if (!starts && a >= z) continue;
+    const int a = starts ? s : max(t0, s + W - 1);   // the tokens done here: [a, z)
+    const int z = starts ? min(e, max(t1, s + W - 1)) : min(e, t1);
+    if (a >= z) return;
 
     ConvWindow<T, V, W> win;
     if (starts) {
-      const long long slot = slot_of(p.slots, p.slots_is64, i, p.pool, p.status, reporter);
+      const long long slot = slot_of(p.slots, p.slots_is64, i, p.pool, p.status, d == 0);
       const bool carried = p.state && slot >= 0 && (!p.has_state || p.has_state[i]);
-      Pack<T, V> old[W - 1];
 #pragma unroll
       for (int k = 0; k < W - 1; ++k) {
-        old[k].zero();
+        Pack<T, V> old;
+        old.zero();
         if (carried)
-          old[k].load(static_cast<const T*>(p.state) + (slot * (W - 1) + k) * p.channels + d);
-        win.set(k, old[k]);
+          old.load(static_cast<const T*>(p.state) + (slot * (W - 1) + k) * p.channels + d);
+        win.set(k, old);
       }
-      if (slot >= 0) {
-        const long long len = e - s;
+      if (slot >= 0) {   // (longer than the window: the last rows are tokens)
         T* ns = static_cast<T*>(p.new_state) + slot * (W - 1) * p.channels + d;
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) {
-          const long long pos = len - (W - 1) + k;   // row k holds this position of the tokens
-          T* to = ns + static_cast<long long>(k) * p.channels;
-          if (pos >= 0) {
-            Pack<T, V> v;
-            v.load(x + (s + pos) * p.x_stride);
-            v.store(to);
-          }
-#pragma unroll
-          for (int j = k; j < W - 1; ++j)   // an old row, in a sequence shorter than the window
-            if (pos + W - 1 == j) old[j].store(to);
+          Pack<T, V> v;
+          v.load(x + static_cast<long long>(e - (W - 1) + k) * p.x_stride);
+          v.store(ns + static_cast<long long>(k) * p.channels);
         }
       }
     } else {
@@ -225,11 +290,11 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
     }
     T* dst = out + a * p.out_stride;
 #pragma unroll 8
-    for (long long t = a; t < z; ++t) {
+    for (int t = a; t < z; ++t) {
       win.row(taps, row_at(t), p.silu).store(dst);
       dst += p.out_stride;
     }
-  }
+  });
 }
 
 // Single tokens: one row per batch entry, its window in the pool.  64 rows of 8192

@@ -269,7 +269,8 @@ int gdn_b200_prefill_static(const void* q, const void* k, const void* v, const f
  *   state        [pool_size, W-1, channels] (oldest row first), NULL = zero
  *   new_state    the same shape: the last W-1 rows of u; may be `state`
  *   has_state    [N] bytes or NULL: sequences whose byte is 0 start from zero
- * output must not overlap x.  activation: GDN_B200_ACT_NONE or _SILU.
+ * output must not overlap x; total_tokens is at most 2^30.  activation:
+ * GDN_B200_ACT_NONE or _SILU.
  */
 int gdn_b200_short_conv(const void* x, int64_t x_stride, const void* weight, const void* bias,
                         const void* state, const void* cu_seqlens, int32_t cu_seqlens_is_int64,

@@ -48,6 +48,7 @@ def _add(lib, rows=2, width=128, eps=1e-6, dtype=0):
     (_conv, dict(channels=0), b"channels"), (_conv, dict(dtype=3), b"dtype"),
     (_conv, dict(act=2), b"activation"), (_conv, dict(t=-1), b"extents"),
     (_conv, dict(n=-1), b"num_seqs"), (_conv, {}, b"null"),
+    (_conv, dict(t=2 ** 30 + 1), b"total_tokens"),
     (_conv_step, dict(width=7), b"width"), (_conv_step, dict(b=-1), b"extents"),
     (_conv_step, {}, b"null"),
     (_scan, dict(P=96), b"head_dim"), (_scan, dict(N=32), b"state_dim"),

@@ -90,6 +90,27 @@ def test_short_conv_strides_pool_and_flags(channels, stride, dtype):
     status_clean()
 
 
+@pytest.mark.parametrize("lens", [[17, 16, 15, 300, 1, 1, 0, 3], [2] * 40 + [90] + [1] * 5,
+                                  [200] + [1] * 63, [0] * 70, [16] * 9])
+@pytest.mark.parametrize("channels", [520, 77])
+def test_short_conv_short_beside_long(lens, channels):
+    """Sequences on either side of the length up to which one thread does them whole."""
+    T, n = sum(lens), len(lens)
+    x, w = rand(T, channels, dtype=BF), rand(channels, 4, dtype=BF)
+    st = rand(n + 4, 3, channels, dtype=BF, seed=2)
+    slots = torch.randperm(n + 4, generator=torch.Generator().manual_seed(n))[:n].cuda()
+    slots[n // 2] = -1
+    cu = offsets(lens)
+    out, ns = torch.full_like(x, float("nan")), st.clone()
+    M.gdn_short_conv(x, w, None, st, cu, out, ns, state_indices=slots)
+    want, pool, mag = O.short_conv(x, w, None, st, cu, st, "silu", slots)
+    check(out, want, mag, CONV_REL, "output")
+    assert torch.equal(ns.double().cpu(), pool)
+    M.gdn_short_conv(x, w, None, st, cu, again := torch.empty_like(x), st, state_indices=slots)
+    assert torch.equal(again, out) and torch.equal(st, ns)
+    status_clean()
+
+
 def test_short_conv_new_prompts_and_uncovered_tokens():
     x, w = rand(50, 64, dtype=BF), rand(64, 4, dtype=BF)
     cu = torch.tensor([5, 20, 41], dtype=torch.int32).cuda()
