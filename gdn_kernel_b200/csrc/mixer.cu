@@ -230,12 +230,20 @@ int scan_setup() {
 
 // How a call's sequences are divided.  A CTA runs 64 columns of a head, one per
 // SM; its start costs about as much as two or three chunks.
-//  * One sequence: as many equal pieces as fill the SMs once.  8,192 tokens of 64
-//    heads run in two pieces; five pieces, with their start-ups, took longer.
+//  * One sequence: as many equal pieces as fill the SMs once, of two chunks at
+//    least.  8,192 tokens of 64 heads run in two pieces; five pieces, with their
+//    start-ups, took longer.  1,024 tokens of 8 heads take 14 us in pieces of two
+//    chunks, 18 of four, 20 of eight.
 //  * Several: a piece is an SM's share of all chunks, so that a sequence that is
-//    longer than that cannot hold up the rest, and most are not divided.
-// The parts of pieces whose states the first kernel makes fill the SMs likewise.
-constexpr int kScanSms = 148, kScanMinPiece = 4, kScanMaxDivided = 1024, kScanMaxParts = 4;
+//    longer than that cannot hold up the rest, and most are not divided.  Where
+//    whole sequences fill half of the SMs, of six chunks at least, as a piece of one
+//    or two left over costs a start (4 sequences of 700 tokens: 32 heads, 21 us whole
+//    and 31 divided; 8 heads, 19 whole and 16 divided).
+// The states of long pieces are made in parts that fill the SMs likewise; in short
+// ones a part's start and its sum cost more (32 heads, sequences of 1400, 100 and
+// 50 tokens: 22 us with one part, 31 with four).
+constexpr int kScanSms = 148, kScanMinPiece = 2, kScanMinPieceFilled = 6;
+constexpr int kScanMaxDivided = 1024, kScanPartedPiece = 16, kScanMaxParts = 4;
 
 struct ScanPlan {
   int seg_chunks;        // 0: not divided
@@ -255,11 +263,13 @@ ScanPlan scan_plan(long long seqs, long long tokens, int heads, int head_dim, in
     const long long pieces = std::max<long long>(1, kScanSms / units);
     piece = (chunks + pieces - 1) / pieces;
   }
-  piece = std::max<long long>(piece, kScanMinPiece);
+  const bool filled = seqs > 1 && seqs * units * 2 > kScanSms;
+  piece = std::max<long long>(piece, filled ? kScanMinPieceFilled : kScanMinPiece);
   if (chunks <= piece) return plan;
   const long long whole = seqs == 1 ? (chunks - 1) / piece : 1;   // pieces whose states are needed
-  plan.parts = static_cast<int>(
-      std::min<long long>(kScanMaxParts, std::max<long long>(1, kScanSms / (units * whole))));
+  if (piece >= kScanPartedPiece)
+    plan.parts = static_cast<int>(
+        std::min<long long>(kScanMaxParts, std::max<long long>(1, kScanSms / (units * whole))));
   piece = (piece + plan.parts - 1) / plan.parts * plan.parts;
   plan.seg_chunks = static_cast<int>(piece);
   plan.max_full = (chunks + seqs) / piece;

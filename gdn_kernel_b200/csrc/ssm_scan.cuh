@@ -575,24 +575,23 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     tmem_alloc(tmem_ptr, 512);
     tmem_relinquish();
   }
-  if (warp == 1 && lane == 0) {
-    *abort_flag = 0;
-#pragma unroll 1
-    for (int i = 0; i < kBCount; ++i) {
-      int n = 1;
-      if (i == kBEmpty || i == kBEmpty + 1) n = 1 + 4;   // products, output warps
-      else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 24;
-      else if (i == kBXwFull || i == kBMFull || i == kBSEmpty) n = 8;
-      else if (i == kBYEmpty ||
-               i == kBHFull || i == kBDsEmpty)
-        n = 4;
-      mbar_init(bars + i, n);
+  if (warp == 1) {   // a barrier per lane
+    const int i = lane;
+    int n = 1;
+    if (i == kBEmpty || i == kBEmpty + 1) n = 1 + 4;   // products, output warps
+    else if (i == kBGateEmpty || i == kBGateEmpty + 1) n = 24;
+    else if (i == kBXwFull || i == kBMFull || i == kBSEmpty) n = 8;
+    else if (i == kBYEmpty || i == kBHFull || i == kBDsEmpty) n = 4;
+    if (i < kBCount) mbar_init(bars + i, n);
+    if (lane == 31) {
+      *abort_flag = 0;
+      prefetch_tmap(&tm_x);
+      prefetch_tmap(&tm_b);
+      prefetch_tmap(&tm_c);
     }
     fence_mbarrier_init();
-    prefetch_tmap(&tm_x);
-    prefetch_tmap(&tm_b);
-    prefetch_tmap(&tm_c);
   }
+  static_assert(kBCount <= 31, "a lane each");
   if (warp == 2) scan_item(sp, blockIdx.y, reinterpret_cast<ScanItem*>(smem + kScItem));
   tc_fence_before();
   __syncthreads();

@@ -301,6 +301,26 @@ def test_scan_weak_decay_over_pieces():
     check(ns1, wp, pmag, PROMPT_STATE_REL, "state")
 
 
+def test_scan_pieces_in_parts():
+    """70 column units, so a sequence runs in two pieces of 17 chunks, each one's state
+    made in two parts; in place."""
+    H, T = 70, 34 * 128 - 31
+    assert M.ssm_prefill_workspace_bytes(1, T, H, 64, 64) > 0
+    x, dt, A_log, B, C, D, bias = scan_inputs(T, H, 64, 1, 64, seed=41)
+    st = rand(1, H, 64, 64, seed=42)
+    cu, out, ns = offsets([T]), torch.empty(T, H, 64, dtype=BF).cuda(), torch.empty_like(st)
+    M.gdn_ssm_prefill(x, dt, A_log, B, C, D, bias, st, cu, out, ns)
+    heads = [0, 33, 69]                      # the oracle on a few of the heads
+    few = (x[:, heads], dt[:, heads], A_log[heads], B, C, D[heads], bias[heads], st[:, heads])
+    want, wp, mag, pmag = O.scan(*few, cu, ns[:, heads])
+    check(out[:, heads], want, mag, PROMPT_REL, "output")
+    check(ns[:, heads], wp, pmag, PROMPT_STATE_REL, "state")
+    again = torch.empty_like(out)
+    M.gdn_ssm_prefill(x, dt, A_log, B, C, D, bias, st, cu, again, st)
+    assert torch.equal(again, out) and torch.equal(st, ns)
+    status_clean()
+
+
 def test_scan_without_skip_and_bias():
     x, dt, A_log, B, C, _, _ = scan_inputs(150, 4, 64, 1, 64)
     dt = dt - 3
