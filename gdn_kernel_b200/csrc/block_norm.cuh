@@ -10,8 +10,8 @@
 // 2048 with an fp32 residual and both norms: 35 us, 5.7 TB/s; a plain copy reaches
 // 6.5): each element is read once, kept in registers between the
 // sum of squares and the scaling, and written once.  Sums are fp32.  `kTeam`
-// threads share a group (part of a warp, a warp, or a block), each holding
-// kVecs 16-byte vectors of every operand.  Rows that no such shape fits (sizes
+// threads share a group (part of a warp, a warp, or with kTeam = 0 the block, as
+// large as the group needs), each holding kVecs 16-byte vectors of every operand.  Rows that no such shape fits (sizes
 // or addresses off 16 bytes) take one element per access and read their
 // operands again, from L1 or L2, after the sum.
 #pragma once
@@ -38,18 +38,21 @@ struct NormParams {
   float eps, scale, weight_offset;
 };
 
-// Sum over the kTeam threads that share a group.
+// Sum over the threads that share a group: kTeam of them, or the block (kTeam = 0).
 template <int kTeam>
 __device__ __forceinline__ float team_sum(float v, float* smem) {
+  constexpr bool kBlock = kTeam == 0;
 #pragma unroll
-  for (int o = (kTeam < 32 ? kTeam : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (kTeam > 32) {
+  for (int o = (kBlock ? 32 : kTeam) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (kBlock) {
     __syncthreads();   // an earlier sum's readers are done
     if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = 0.0f;
+    // every warp adds the warps' sums, in the same order
+    const int lane = threadIdx.x & 31;
+    v = lane < static_cast<int>(blockDim.x >> 5) ? smem[lane] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kTeam / 32; ++i) v += smem[i];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   }
   return v;
 }
@@ -71,16 +74,19 @@ __device__ __forceinline__ void apply_gate(float (&v)[V], const Pack<T, V>& gate
 }
 
 constexpr int kNormThreads = 128;   // of a block, where a team is a warp or less
+constexpr int kNormBlock = 1024;    // largest block of one team
 
 template <typename T, int V, int kTeam, int kVecs>
-__global__ void __launch_bounds__(kTeam > 32 ? kTeam : kNormThreads)
+__global__ void __launch_bounds__(kTeam > 0 ? kNormThreads : kVecs == 1 ? 512 : kNormBlock)
 gdn_gated_norm_kernel(const NormParams p) {
-  constexpr int kTeams = (kTeam > 32 ? kTeam : kNormThreads) / kTeam;
   __shared__ float smem[32];
-  const int lane = threadIdx.x % kTeam;
+  const int team = kTeam > 0 ? kTeam : static_cast<int>(blockDim.x);
+  const int lane = kTeam > 0 ? threadIdx.x % (kTeam > 0 ? kTeam : 1) : threadIdx.x;
   // 32 bits: groups stay below 2^31, and a 64-bit division took 10 of 48 us at 8192
   // rows of 32 groups of 128
-  const unsigned int id = blockIdx.x * kTeams + threadIdx.x / kTeam;
+  const unsigned int id =
+      kTeam > 0 ? blockIdx.x * (kNormThreads / (kTeam > 0 ? kTeam : 1)) + threadIdx.x / (kTeam > 0 ? kTeam : 1)
+                : blockIdx.x;
   const bool live = id < static_cast<unsigned int>(p.rows * p.per_row);
   const unsigned int row = id / p.per_row;
   const int c0 = static_cast<int>(id - row * p.per_row) * p.group;
@@ -92,7 +98,7 @@ gdn_gated_norm_kernel(const NormParams p) {
   Pack<T, V> xv[kVecs], gv[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int c = (lane + i * kTeam) * V;
+    const int c = (lane + i * team) * V;
     xv[i].zero();
     gv[i].zero();
     if (live && c < p.group) {
@@ -111,7 +117,7 @@ gdn_gated_norm_kernel(const NormParams p) {
   const float inv = rsqrtf(team_sum<kTeam>(ss, smem) * p.inv_group + p.eps);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int c = (lane + i * kTeam) * V;
+    const int c = (lane + i * team) * V;
     if (!live || c >= p.group) continue;
     float y[V];
 #pragma unroll
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_any_kernel(const NormParam
     if (g && !p.norm_first) v *= gate_act(to_float(g[c]), p.silu);
     ss = fmaf(v, v, ss);
   }
-  const float inv = rsqrtf(team_sum<256>(ss, smem) * p.inv_group + p.eps);
+  const float inv = rsqrtf(team_sum<0>(ss, smem) * p.inv_group + p.eps);
   for (int c = threadIdx.x; c < p.group; c += 256) {
     float v = to_float(x[c]);
     const float a = g ? gate_act(to_float(g[c]), p.silu) : 1.0f;
@@ -196,12 +202,15 @@ struct ResidualVec {
 };
 
 template <typename T, typename R, int V, int kTeam, int kVecs>
-__global__ void __launch_bounds__(kTeam > 32 ? kTeam : kNormThreads)
+__global__ void __launch_bounds__(kTeam > 0 ? kNormThreads : kVecs == 1 ? 512 : kNormBlock)
 gdn_add_norm_kernel(const NormParams p) {
-  constexpr int kThreads = kTeam > 32 ? kTeam : kNormThreads;
   __shared__ float smem[32];
-  const int lane = threadIdx.x % kTeam;
-  const long long id = static_cast<long long>(blockIdx.x) * (kThreads / kTeam) + threadIdx.x / kTeam;
+  const int team = kTeam > 0 ? kTeam : static_cast<int>(blockDim.x);
+  const int lane = kTeam > 0 ? threadIdx.x % (kTeam > 0 ? kTeam : 1) : threadIdx.x;
+  const long long id = kTeam > 0 ? static_cast<long long>(blockIdx.x) *
+                                           (kNormThreads / (kTeam > 0 ? kTeam : 1)) +
+                                       threadIdx.x / (kTeam > 0 ? kTeam : 1)
+                                 : blockIdx.x;
   const bool live = id < p.rows;
   const long long row = live ? id : 0;
   const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
@@ -213,7 +222,7 @@ gdn_add_norm_kernel(const NormParams p) {
   ResidualVec<T, R, V> rv[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int c = (lane + i * kTeam) * V;
+    const int c = (lane + i * team) * V;
     xv[i].zero();
     rv[i].zero();
     if (live && c < p.width) {
@@ -236,7 +245,7 @@ gdn_add_norm_kernel(const NormParams p) {
   float rf[kVecs][V], ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int c = (lane + i * kTeam) * V;
+    const int c = (lane + i * team) * V;
     float f[V];
     xv[i].unpack(f);
     rv[i].unpack(rf[i]);
@@ -268,7 +277,7 @@ gdn_add_norm_kernel(const NormParams p) {
   const float inv = rsqrtf(team_sum<kTeam>(ss, smem) * p.inv_width + p.eps);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int c = (lane + i * kTeam) * V;
+    const int c = (lane + i * team) * V;
     if (!live || c >= p.width) continue;
     Pack<T, V> wv;
     float wf[V], y[V];
@@ -294,7 +303,7 @@ __global__ void __launch_bounds__(256) gdn_add_norm_any_kernel(const NormParams 
   if (bw) {
     float ss = 0.0f;
     for (int c = threadIdx.x; c < p.width; c += 256) ss = fmaf(to_float(x[c]), to_float(x[c]), ss);
-    binv = rsqrtf(team_sum<256>(ss, smem) * p.inv_width + p.eps);
+    binv = rsqrtf(team_sum<0>(ss, smem) * p.inv_width + p.eps);
   }
   // r' by element, from the operands: nr may be r, so r' is formed twice before it is stored
   auto sum = [&](int c) {
@@ -307,7 +316,7 @@ __global__ void __launch_bounds__(256) gdn_add_norm_any_kernel(const NormParams 
     const float v = sum(c);
     ss = fmaf(v, v, ss);
   }
-  const float inv = rsqrtf(team_sum<256>(ss, smem) * p.inv_width + p.eps);
+  const float inv = rsqrtf(team_sum<0>(ss, smem) * p.inv_width + p.eps);
   for (int c = threadIdx.x; c < p.width; c += 256) {
     const float v = sum(c);
     nr[c] = from_float<R>(v);

@@ -104,12 +104,15 @@ int check_conv(int64_t rows, int64_t pool, int32_t channels, int32_t width, int3
 }
 
 // ------------------------------------------------------------ norms
+// Threads of a block that is one team: whole warps, as many as the vectors need.
+unsigned team_threads(int nv, int vecs) { return static_cast<unsigned>((nv + 32 * vecs - 1) / (32 * vecs) * 32); }
+
 template <typename T, int kTeam, int kVecs>
 void launch_gated(const NormParams& p, long long groups, cudaStream_t st) {
-  constexpr int per_block = kTeam > 32 ? 1 : kNormThreads / kTeam;
+  constexpr int per_block = kTeam > 0 ? kNormThreads / (kTeam > 0 ? kTeam : 1) : 1;
   gdn_gated_norm_kernel<T, kLanes<T>, kTeam, kVecs>
       <<<static_cast<unsigned>((groups + per_block - 1) / per_block),
-         kTeam > 32 ? kTeam : kNormThreads, 0, st>>>(p);
+         kTeam > 0 ? kNormThreads : team_threads(p.group / kLanes<T>, kVecs), 0, st>>>(p);
 }
 
 template <typename T>
@@ -120,29 +123,26 @@ int gated_call(const NormParams& p, cudaStream_t st) {
   const bool wide = p.group % kLanes<T> == 0 && wide_rows(p.x, p.x_stride, size) &&
                     (!p.gate || wide_rows(p.gate, p.gate_stride, size)) &&
                     wide_rows(p.out, p.out_stride, size) && aligned(p.weight, 16);
-  // A vector of each operand per thread as far as a block goes: more per thread
-  // was slower at every width tried (2048 wide: 35 us with one, 40 with four, 48
-  // with eight), as fewer warps then hide the sum.
+  // A vector of each operand per thread up to 512 threads: more per thread was
+  // slower (2048 wide: 35 us with one, 40 with four, 48 with eight), as fewer warps
+  // then hide the sum.
   const int nv = p.group / kLanes<T>;
   if (!wide || nv > 4096) gdn_gated_norm_any_kernel<T><<<static_cast<unsigned>(groups), 256, 0, st>>>(p);
   else if (nv <= 8) launch_gated<T, 8, 1>(p, groups, st);
   else if (nv <= 16) launch_gated<T, 16, 1>(p, groups, st);
   else if (nv <= 32) launch_gated<T, 32, 1>(p, groups, st);
-  else if (nv <= 64) launch_gated<T, 64, 1>(p, groups, st);
-  else if (nv <= 128) launch_gated<T, 128, 1>(p, groups, st);
-  else if (nv <= 256) launch_gated<T, 256, 1>(p, groups, st);
-  else if (nv <= 512) launch_gated<T, 512, 1>(p, groups, st);
-  else if (nv <= 1024) launch_gated<T, 512, 2>(p, groups, st);
-  else launch_gated<T, 1024, 4>(p, groups, st);
+  else if (nv <= 512) launch_gated<T, 0, 1>(p, groups, st);
+  else if (nv <= 2048) launch_gated<T, 0, 2>(p, groups, st);
+  else launch_gated<T, 0, 4>(p, groups, st);
   return launched("gated norm launch");
 }
 
 template <typename T, typename R, int kTeam, int kVecs>
 void launch_add(const NormParams& p, cudaStream_t st) {
-  constexpr int per_block = kTeam > 32 ? 1 : kNormThreads / kTeam;
+  constexpr int per_block = kTeam > 0 ? kNormThreads / (kTeam > 0 ? kTeam : 1) : 1;
   gdn_add_norm_kernel<T, R, kLanes<T>, kTeam, kVecs>
       <<<static_cast<unsigned>((p.rows + per_block - 1) / per_block),
-         kTeam > 32 ? kTeam : kNormThreads, 0, st>>>(p);
+         kTeam > 0 ? kNormThreads : team_threads(p.width / kLanes<T>, kVecs), 0, st>>>(p);
 }
 
 template <typename T, typename R>
@@ -158,12 +158,9 @@ int add_call(const NormParams& p, cudaStream_t st) {
   const int nv = p.width / kLanes<T>;
   if (!wide || nv > 4096) gdn_add_norm_any_kernel<T, R><<<static_cast<unsigned>(p.rows), 256, 0, st>>>(p);
   else if (nv <= 32) launch_add<T, R, 32, 1>(p, st);
-  else if (nv <= 64) launch_add<T, R, 64, 1>(p, st);
-  else if (nv <= 128) launch_add<T, R, 128, 1>(p, st);
-  else if (nv <= 256) launch_add<T, R, 256, 1>(p, st);
-  else if (nv <= 512) launch_add<T, R, 512, 1>(p, st);
-  else if (nv <= 1024) launch_add<T, R, 512, 2>(p, st);
-  else launch_add<T, R, 1024, 4>(p, st);
+  else if (nv <= 512) launch_add<T, R, 0, 1>(p, st);
+  else if (nv <= 2048) launch_add<T, R, 0, 2>(p, st);
+  else launch_add<T, R, 0, 4>(p, st);
   return launched("add norm launch");
 }
 
