@@ -37,8 +37,8 @@
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
 // there, so nothing of them (not even a NaN) enters a product's sum.
 //
-// Measured: 8192 tokens, 64 heads of 64, state 128, 99 us with the kernel of the
-// pieces' states (20 us); 20011 ragged tokens of 32 heads of 128, state 64, 173 us.
+// Measured: 8192 tokens, 64 heads of 64, state 128, 98 us with the kernel of the
+// pieces' states (20 us); 20011 ragged tokens of 32 heads of 128, state 64, 161 us.
 // A chunk takes about 4000 clocks, its shared-memory traffic 3070 (384 KB: 208 of
 // product operands, 80 of arriving tiles, 96 of x, w X and h), the tensor pipe is
 // active for 2750; the rest is handing over.  128 tokens a chunk, because products
@@ -206,17 +206,18 @@ __device__ inline void scan_item(const ScanParams& sp, int item, ScanItem* out) 
   *out = it;
 }
 
-// Waits are warp-uniform and bounded: so many tries, each of which may sleep a
-// microsecond, some tens of milliseconds at least and about a second at most.
-// The first to run out raises the abort flag, which ends every role's loop.
-// (A count takes a fraction of the code of a clock, and the roles' loops have to
-// fit the instruction cache together.)
-constexpr int kScanWaitTries = 1 << 20;
+// Waits are warp-uniform and bounded: so many tries, each of which sleeps up to 4 us
+// (without a hint; one of a microsecond made the whole 2-3 % slower), so half a second
+// at most and milliseconds at the least.  None spans more than a few chunks' work.
+// The first to run out raises the abort flag, which ends every role's loop.  (A count
+// takes a fraction of the code of a clock, and the roles' loops have to fit the
+// instruction cache together.)
+constexpr int kScanWaitTries = 1 << 17;
 __device__ __forceinline__ bool scan_try_wait(uint32_t addr, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(addr), "r"(parity)
@@ -618,6 +619,11 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   };
   constexpr int kSteps = N / 16;   // k-steps over the state dimension
 
+  // The kernel before made the states of pieces.  This one may have started beside
+  // it (programmatic launch); what needs them waits here, all of it, so that no
+  // bounded wait below depends on how long that kernel takes.
+  if (it.pieces > 1 && (it.piece > 0 || p.state == p.new_state))
+    asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nch == 0) {
     if (it.seq >= 0) {   // an empty sequence: nothing but the state
       bool carried;
@@ -832,10 +838,6 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     };
     bool carried;
     const long long slot = find_state(carried);
-    // The kernel before made the states of pieces; this one may have started
-    // beside it (programmatic launch), and only here needs it to be done.
-    if (it.pieces > 1 && (it.piece > 0 || p.state == p.new_state))
-      asm volatile("griddepcontrol.wait;" ::: "memory");
     if (state_row) {   // the start: what the pieces before this one leave, and the carried state
       float log_decay = 0.0f;
       const long long row0 = static_cast<long long>(it.first_row) * sp.parts;
