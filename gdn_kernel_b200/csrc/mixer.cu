@@ -422,7 +422,11 @@ extern "C" int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const v
 extern "C" uint64_t gdn_b200_ssm_prefill_workspace_size(int64_t num_seqs, int64_t total_tokens,
                                                         int32_t num_heads, int32_t head_dim,
                                                         int32_t state_dim) {
-  if (num_seqs <= 0 || total_tokens <= 0 || num_heads <= 0 || head_dim <= 0 || state_dim <= 0)
+  // sizes that gdn_b200_ssm_prefill refuses need nothing (and have no plan: a head of
+  // less than kScanCols columns is no unit)
+  if (num_seqs <= 0 || num_seqs > 65535 || total_tokens <= 0 || total_tokens > kMaxGrid - kScanQ ||
+      num_heads <= 0 || num_heads > 65535 || (head_dim != 64 && head_dim != 128) ||
+      (state_dim != 64 && state_dim != 128))
     return 0;
   return scan_plan(num_seqs, total_tokens, num_heads, head_dim, state_dim).bytes;
 }

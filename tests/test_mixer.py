@@ -78,6 +78,18 @@ def test_nothing_to_do_is_no_error(fn, kw):
     assert lib.gdn_b200_last_error() == b""
 
 
+@pytest.mark.parametrize("seqs,tokens,H,P,N", [
+    (1, 512, 8, 1, 64), (1, 512, 8, 32, 64), (1, 512, 8, 63, 128), (1, 512, 8, 96, 64),
+    (1, 512, 8, 256, 64), (1, 512, 8, 64, 32), (1, 512, 8, 64, 0), (1, 512, 0, 64, 64),
+    (1, 512, 70000, 64, 64), (0, 512, 8, 64, 64), (-1, 512, 8, 64, 64), (70000, 2 ** 20, 8, 64, 64),
+    (1, 2 ** 40, 8, 64, 64), (1, -5, 8, 64, 64)])
+def test_workspace_of_refused_sizes_is_nothing(seqs, tokens, H, P, N):
+    lib = _lib.load()
+    assert lib.gdn_b200_ssm_prefill_workspace_size(seqs, tokens, H, P, N) == 0
+    assert M.ssm_prefill_workspace_bytes(seqs, tokens, H, P, N) == 0
+    assert M.ssm_prefill_workspace_bytes(1, 512, 8, 64, 64) > 0
+
+
 BF = torch.bfloat16
 
 
@@ -175,6 +187,13 @@ F32, I32, I64 = torch.float32, torch.int32, torch.int64
 def test_python_refuses(call, kw, words):
     with pytest.raises(ValueError, match=words):
         call(**kw)
+
+
+@pytest.mark.parametrize("P", [1, 32, 63])
+def test_python_refuses_small_heads_before_planning(P):
+    with pytest.raises(ValueError, match="head_dim"):
+        scan(x=z(512, 2, P), dt=z(512, 2), B=z(512, 1, 128), C=z(512, 1, 128), output=z(512, 2, P),
+             cu=torch.tensor([0, 512], dtype=torch.int32))
 
 
 # ------------------------------------------------------------------ the oracle
