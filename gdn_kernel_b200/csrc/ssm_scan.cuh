@@ -813,8 +813,13 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         if (b == top && c > 0) ok = wait(kBYFull, c - 1, kStatusMmaTimeout);   // the last M is read
         if (ok) tmem_st16(tmem + kTmM + 16 * b + tm_lane, m);
       }
+      // The warp without a block waits like the others: its arrival for this chunk must
+      // not stand in for one of the last chunk's that is still to come.
+      if (top < 0) {
+        arrive(kBSEmpty);
+        ok = c == 0 || wait(kBYFull, c - 1, kStatusMmaTimeout);
+      }
       if (!ok) break;
-      if (top < 0) arrive(kBSEmpty);
       tmem_wait_st();
       tc_fence_before();
       arrive(kBMFull);
