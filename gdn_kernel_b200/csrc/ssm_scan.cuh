@@ -147,7 +147,8 @@ struct ScanItem {
 
 // The piece of grid row `item`.  Whole pieces come first, so that the long work
 // starts first: row r is the r-th whole piece over all sequences, found by a
-// running sum, 32 sequences at a time, by one warp.
+// running sum, 32 sequences at a time, by one warp.  A sequence of bad offsets, or
+// whose pieces do not fit the grid and the workspace, is reported and skipped.
 __device__ inline void scan_item(const ScanParams& sp, int item, ScanItem* out) {
   const SsmParams& p = sp.s;
   const int lane = threadIdx.x & 31;
@@ -192,7 +193,9 @@ __device__ inline void scan_item(const ScanParams& sp, int item, ScanItem* out) 
   it.t_begin = begin;
   it.len = len;
   it.first_row = first_row;
-  if (seq >= 0 && len < 0) {
+  // Offsets that fall and rise again can hold more whole pieces than the tokens
+  // account for, and the workspace has rows for no more than those.
+  if (seq >= 0 && (len < 0 || first_row + full > sp.max_full)) {
     atomicOr(p.status, kMixerBadSeqlens);
     it.seq = -1;
   }

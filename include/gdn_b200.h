@@ -258,7 +258,8 @@ int gdn_b200_prefill_static(const void* q, const void* k, const void* v, const f
  * written by one call must be distinct, and none may be read by another entry.
  * New states may be written in place.  Offsets that do not rise within
  * [0, total_tokens] raise GDN_B200_STATUS_BAD_SEQLENS; such sequences are
- * skipped.  Tokens outside [cu_seqlens[0], cu_seqlens[N]) are not written.
+ * skipped, and where offsets return to earlier tokens so may be those that
+ * follow.  Tokens outside [cu_seqlens[0], cu_seqlens[N]) are not written.
  */
 
 /*

@@ -365,6 +365,29 @@ def test_scan_bad_offsets_and_slots():
     assert _lib.device_status(dev) == _lib.STATUS_BAD_INDEX
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_scan_unordered_offsets_stay_in_the_workspace(in_place):
+    """Offsets that return to the start: the first sequence takes the workspace that
+    8192 tokens account for (16 pieces of 4 chunks, 17 rows), the later ones are skipped.
+    What lies behind the workspace is NaN, and is neither read nor written."""
+    H, P, N, T = 8, 64, 128, 8192
+    ins = scan_inputs(T, H, P, 1, N, seed=51)
+    cu = torch.tensor([0, T] * 4, dtype=torch.int32).cuda()
+    need = M.ssm_prefill_workspace_bytes(7, T, H, P, N)
+    assert need == 17 * (2 * H * P * N * 4 + H * 4)
+    ws = torch.full((4 * need // 4,), float("nan"), device="cuda")
+    st = rand(7, H, P, N, std=0.5, seed=52)
+    base = st.clone()
+    ns = st if in_place else st.clone()
+    out = torch.empty(T, H, P, dtype=BF).cuda()
+    M.gdn_ssm_prefill(*ins, st, cu, out, ns, workspace=ws.view(torch.uint8)[:need])
+    assert _lib.device_status(torch.cuda.current_device()) == _lib.STATUS_BAD_SEQLENS
+    want, wp, mag, pmag = O.scan(*ins, base[:1], cu[:2], base[:1])
+    check(out, want, mag, PROMPT_REL, "output")
+    check(ns[:1], wp, pmag, PROMPT_STATE_REL, "state")
+    assert torch.equal(ns[1:], base[1:]) and ws[need // 4:].isnan().all()
+
+
 @pytest.mark.parametrize("P,N", [(64, 64), (64, 128), (128, 64), (128, 128)])
 @pytest.mark.parametrize("batch,H,G", [(1, 4, 1), (5, 6, 3), (33, 2, 2)])
 def test_scan_step(P, N, batch, H, G):
