@@ -423,8 +423,10 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
   const uint32_t tmem = static_cast<uint32_t>(warp_uniform(static_cast<int>(*tmem_ptr)));
   const int t_last = warp_uniform(it.t_begin + (c0 + nch - 1) * kScanQ);
   const ScanSync sync{smem_u32(bars), abort_flag};
-  // Chunk i of the order, from the end: false once the decays leave nothing of it.
-  auto more = [&](int i) { return later[2 * (i & 1)] > kScanGone; };
+  // Whether a chunk counts after decays of `log_decay`: not once they leave nothing of
+  // it, nor after a NaN, which the state then holds already.  All roles end by this.
+  auto counts = [](float log_decay) { return log_decay > kScanGone; };
+  auto more = [&](int i) { return counts(later[2 * (i & 1)]); };   // chunk i, from the end
 
   // the scan's blocks may take the SMs that this grid leaves or has done with
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -493,7 +495,7 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
       if (i > 0) {
         if (!sync.wait(kAGateFull + (st ^ 1), (i - 1) >> 1, kStatusMmaTimeout)) break;
         done = later[2 * (st ^ 1) + 1];
-        ended = later[2 * (st ^ 1)] <= kScanGone;
+        ended = !more(i - 1);
       }
       if (i >= 2 && !sync.wait(kAGateEmpty + st, (i >> 1) - 1, kStatusMmaTimeout)) break;
       float* g = reinterpret_cast<float*>(smem + kSsGate + st * kScanQ * 4);
@@ -503,11 +505,11 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
       if (lane == 0) {
         later[2 * st] = done;
         later[2 * st + 1] = done + total;
-        if (col0 == 0 && !ended && (i == nch - 1 || done <= kScanGone))
+        if (col0 == 0 && !ended && (i == nch - 1 || !counts(done)))
           sp.seg_decay[static_cast<long long>(blockIdx.y) * p.heads + head] = done + total;
       }
       sync.arrive(kAGateFull + st);
-      if (done <= kScanGone) break;
+      if (!counts(done)) break;
     }
   } else {
     // two warpgroups, one chunk each in turn

@@ -343,6 +343,39 @@ def test_scan_ignores_values_of_other_sequences():
     assert torch.equal(out[70:170], clean[70:170]) and torch.equal(ns[1], cs[1])
 
 
+@pytest.mark.parametrize("where", ["dt", "bias", "A_log"])
+def test_scan_of_pieces_with_a_nan_step(where):
+    """A NaN in the steps of one head, in the last of a piece's 8 chunks, which is the
+    first that its state's kernel takes: that head's outputs and state are NaN from there
+    on (and from its chunk's start at most), everything else is as without it, and no wait
+    runs out.  The head hardly forgets, so that no decay of 0 ends the NaN's reach."""
+    H, lens = 16, [8192, 300]
+    rows = (67 + 2) // 8                       # whole pieces that the workspace holds
+    assert (M.ssm_prefill_workspace_bytes(2, sum(lens), H, 64, 128)
+            == rows * (2 * H * 64 * 128 * 4 + H * 4))
+    ins = list(scan_inputs(sum(lens), H, 64, 1, 128, seed=61))
+    ins[2][3] = -9.0
+    cu, at = offsets(lens), 15 * 128 + 50
+    clean, cs = M.ssm_prefill(*ins, None, cu)
+    k = {"dt": 1, "A_log": 2, "bias": 6}[where]
+    ins[k] = ins[k].clone()
+    if where == "dt":
+        ins[k][at, 3] = float("nan")
+    else:
+        ins[k][3] = float("nan")
+    out, ns = M.ssm_prefill(*ins, None, cu)
+    status_clean()
+    others = [h for h in range(H) if h != 3]
+    assert torch.equal(out[:, others], clean[:, others]) and torch.equal(ns[:, others], cs[:, others])
+    assert ns[0, 3].isnan().all()
+    if where == "dt":
+        begin = at // 128 * 128
+        assert torch.equal(out[:begin, 3], clean[:begin, 3]) and out[at:lens[0], 3].isnan().all()
+        assert torch.equal(out[lens[0]:], clean[lens[0]:]) and torch.equal(ns[1], cs[1])
+    else:
+        assert out[:lens[0], 3].isnan().all() and ns[1, 3].isnan().all()
+
+
 def test_scan_of_nothing():
     ins = scan_inputs(0, 4, 64, 1, 128)
     st = rand(2, 4, 64, 128)
