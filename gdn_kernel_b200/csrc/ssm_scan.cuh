@@ -18,9 +18,12 @@
 // more.  The roundings of h and M are 2^-8 of their terms each at most, as in
 // the bf16 output itself.
 //
-// Decays come from sums towards the chunk's end, sfx_t = L_Q - L_t, which are
-// small and hence accurate exactly where w is not; M and e^L only need the
-// accuracy of bf16.  All exponents are in base 2.  M's 32 x 32 blocks below the
+// Decays come from sums over blocks of 32 tokens: after a token to its block's end,
+// and of whole blocks.  w and e^L add up such sums, none of them positive, and are
+// small, hence accurate, exactly where the result is not.  The only differences are
+// within a block, of sums that a floor under each token's decay (kScanGone) keeps
+// below 9600: off by 2^-9 at most if all 32 tokens are as steep as that, 2^-16 with
+// sums of 100.  All exponents are in base 2.  M's 32 x 32 blocks below the
 // diagonal ones need no exponential per element: with r the last token of the
 // columns' block, L_t - L_s = (L_t - L_r) + (L_r - L_s), neither part positive,
 // so e^{L_t - L_s} step_s is a row factor times a column factor.
@@ -60,12 +63,12 @@ constexpr int kScanThreads = 896;
 constexpr uint32_t kScanTile = 16384;    // 128 rows x 64 bf16
 
 // Shared memory: two stages of C (two halves of N), B (two halves) and X, the
-// split w X (three tiles), h, the gates and the barriers.
+// split w X (three tiles), h, the gates and the barriers (with the blocks' decays).
 constexpr uint32_t kScC = 0, kScB = 2 * kScanTile, kScX = 4 * kScanTile;
 constexpr uint32_t kScStage = 5 * kScanTile;
 constexpr uint32_t kScXw = 2 * kScStage;
 constexpr uint32_t kScH = kScXw + 3 * kScanTile;
-constexpr uint32_t kScGate = kScH + kScanTile;   // per stage: g[128], sfx[128], v[96] floats
+constexpr uint32_t kScGate = kScH + kScanTile;   // per stage: step[128], end[128], v[96] floats
 constexpr uint32_t kScGateStage = (2 * kScanQ + 96) * 4;
 constexpr uint32_t kScMisc = kScGate + 2 * kScGateStage;
 constexpr uint32_t kScItem = kScMisc + 224;       // barriers and flags before it
@@ -268,24 +271,21 @@ __device__ __forceinline__ float scan_step_size(float v) {
   return v != v ? v : fmaxf(v, 0.0f) + (s + s);
 }
 
-// Accurate to 2^-22 absolutely, which is what a weight's exponent needs.
-__device__ __forceinline__ float scan_log2(float v) {
-  float r;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
+// A weight below this exponent, or a decay, is zero in fp32 whatever the rest.  So no
+// token's decay counts as steeper, which keeps sums of 32 of them near enough to
+// zero for their differences to be accurate, and finite for an infinite step.
+constexpr float kScanGone = -300.0f;
 
 // The gates of chunks by one warp, lane owning one token of each block of 32: the
-// steps, the log2 decays after a token to the chunk's end (sfx), after each
-// block (ref), and of the whole chunk.  A chunk's dt are loaded while the one
-// before it (of this warp) is worked on.
+// steps, the log2 decays after a token to its block's end, and of each block.  A
+// chunk's dt are loaded while the one before it (of this warp) is worked on.
 struct ScanGates {
   const __nv_bfloat16* dt;    // of the piece's first token and this head
   long long stride;
   float a2, bias;             // log2 decay per step, and dt_bias
   int len;                    // tokens of the piece
   __nv_bfloat16 raw[4];
-  float step[4], sfx[4], ref[4], total;
+  float step[4], end[4], block[4];
   __device__ __forceinline__ void fetch(int c) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -309,8 +309,9 @@ struct ScanGates {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       step[b] = scan_step_size(to_float(raw[b]) + bias);
-      if (c * kScanQ + 32 * b + lane >= len) step[b] = 0.0f;
       v[b] = a2 * step[b];
+      if (v[b] < kScanGone) v[b] = kScanGone;   // (a NaN stays)
+      if (c * kScanQ + 32 * b + lane >= len) step[b] = v[b] = 0.0f;
     }
     fetch(next);
 #pragma unroll
@@ -320,13 +321,11 @@ struct ScanGates {
         const float u = __shfl_down_sync(0xffffffffu, v[b], o);
         if (lane + o < 32) v[b] += u;
       }
-    total = 0.0f;
 #pragma unroll
-    for (int b = 3; b >= 0; --b) {
+    for (int b = 0; b < 4; ++b) {
       const float after = __shfl_down_sync(0xffffffffu, v[b], 1);
-      ref[b] = total;
-      sfx[b] = total + (lane == 31 ? 0.0f : after);
-      total += __shfl_sync(0xffffffffu, v[b], 0);
+      end[b] = lane == 31 ? 0.0f : after;
+      block[b] = __shfl_sync(0xffffffffu, v[b], 0);
     }
   }
 };
@@ -357,9 +356,6 @@ __device__ __forceinline__ void scan_scale_row(uint8_t* xw, const uint8_t* x, in
   }
 }
 
-// A weight below this exponent, or a decay, is zero in fp32 whatever the rest.
-constexpr float kScanGone = -300.0f;
-
 // ------------------------------------------------ the states of pieces
 // One CTA per part of a whole piece that is not its sequence's last, and 64
 // columns of a head: the state it adds, sum over its tokens of e^{L_end - L_s} step_s B_s x_s^T,
@@ -368,7 +364,7 @@ constexpr float kScanGone = -300.0f;
 constexpr int kStateThreads = 384;
 constexpr uint32_t kSsB = 0, kSsX = 2 * kScanTile, kSsStage = 3 * kScanTile;
 constexpr uint32_t kSsXw = 2 * kSsStage;                       // two sets of three tiles
-constexpr uint32_t kSsGate = kSsXw + 6 * kScanTile;            // per stage: exponents [128]
+constexpr uint32_t kSsGate = kSsXw + 6 * kScanTile;            // per stage: weights [128]
 constexpr uint32_t kSsMisc = kSsGate + 2 * kScanQ * 4;
 constexpr uint32_t kSsItem = kSsMisc + 208;
 constexpr uint32_t kStateSmem = kSsMisc + 256;
@@ -499,9 +495,12 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
       }
       if (i >= 2 && !sync.wait(kAGateEmpty + st, (i >> 1) - 1, kStatusMmaTimeout)) break;
       float* g = reinterpret_cast<float*>(smem + kSsGate + st * kScanQ * 4);
+      float total = 0.0f;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) g[32 * b + lane] = done + gates.sfx[b] + scan_log2(gates.step[b]);
-      const float total = gates.total;
+      for (int b = 3; b >= 0; --b) {
+        g[32 * b + lane] = gates.step[b] * scan_exp2(done + total + gates.end[b]);
+        total += gates.block[b];
+      }
       if (lane == 0) {
         later[2 * st] = done;
         later[2 * st + 1] = done + total;
@@ -519,7 +518,7 @@ gdn_ssm_piece_state_kernel(const __grid_constant__ CUtensorMap tm_x,
       const int st = i & 1;
       if (!sync.wait(kAGateFull + st, i >> 1, kStatusMmaTimeout)) break;
       const bool go = more(i);
-      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kSsGate + st * kScanQ * 4)[row]);
+      const float w = reinterpret_cast<const float*>(smem + kSsGate + st * kScanQ * 4)[row];
       sync.arrive(kAGateEmpty + st);
       if (!go) break;
       if (!sync.wait(kAFull + st, i >> 1, kStatusTmaTimeout)) break;
@@ -574,8 +573,10 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kScMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kScMisc + 8 * kBCount);
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + kScMisc + 8 * kBCount + 4);
-  float* totals = reinterpret_cast<float*>(smem + kScMisc + 8 * kBCount + 8);   // [2]
-  static_assert(8 * kBCount + 16 <= 224 && sizeof(ScanItem) <= 32, "they fit");
+  float4* blocks = reinterpret_cast<float4*>(smem + kScMisc + 8 * kBCount + 8);   // [2]: decays
+  static_assert(8 * kBCount + 40 <= 224 && (kScMisc + 8 * kBCount + 8) % 16 == 0 &&
+                    sizeof(ScanItem) <= 32,
+                "they fit");
 
   if (warp == 0) {
     tmem_alloc(tmem_ptr, 512);
@@ -750,12 +751,12 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         float* g = reinterpret_cast<float*>(smem + kScGate + st * kScGateStage) + lane;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          // log2 of a zero step is -inf: a padded token has no weight anywhere
-          g[32 * b] = gates.sfx[b] + scan_log2(gates.step[b]);
-          g[kScanQ + 32 * b] = gates.sfx[b];
-          if (b < 3) g[2 * kScanQ + 32 * b] = gates.step[b] * scan_exp2(gates.sfx[b] - gates.ref[b]);
+          g[32 * b] = gates.step[b];
+          g[kScanQ + 32 * b] = gates.end[b];
+          if (b < 3) g[2 * kScanQ + 32 * b] = gates.step[b] * scan_exp2(gates.end[b]);
         }
-        if (lane == 0) totals[st] = gates.total;
+        if (lane == 0)
+          blocks[st] = make_float4(gates.block[0], gates.block[1], gates.block[2], gates.block[3]);
         arrive(kBGateFull + st);
       }
     }
@@ -776,7 +777,8 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       const int st = c & 1;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
       const float* g = reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage);
-      const float mine = g[kScanQ + row];
+      const float* block = reinterpret_cast<const float*>(blocks + st);
+      const float mine = g[kScanQ + row], since = block[quad] - mine;   // from the block's start
       if (!wait(kBSFull, c, kStatusMmaTimeout)) break;
       tc_fence_after();
       bool ok = true;
@@ -786,21 +788,25 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         uint32_t m[16];
         tmem_ld32(tmem + kTmS + 32 * b + tm_lane, s);
         if (b == quad) {
-          const float4* f4 = reinterpret_cast<const float4*>(g + 32 * b);
+          const float4* step4 = reinterpret_cast<const float4*>(g + 32 * b);
+          const float4* end4 = reinterpret_cast<const float4*>(g + kScanQ + 32 * b);
           tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float4 gv = f4[j];
-            const float f[4] = {gv.x, gv.y, gv.z, gv.w};
+            const float4 gv = step4[j], ev = end4[j];
+            const float f[4] = {gv.x, gv.y, gv.z, gv.w}, end[4] = {ev.x, ev.y, ev.z, ev.w};
             float v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)   // a select: a masked S may hold anything
-              v[e] = 4 * j + e <= lane ? s[4 * j + e] * scan_exp2(f[e] - mine) : 0.0f;
+              v[e] = 4 * j + e <= lane ? s[4 * j + e] * (f[e] * scan_exp2(end[e] - mine)) : 0.0f;
             m[2 * j] = pack_bf16x2(v[0], v[1]);
             m[2 * j + 1] = pack_bf16x2(v[2], v[3]);
           }
         } else {
-          const float u = scan_exp2(g[kScanQ + 32 * b + 31] - mine);
+          float after = since;   // and the blocks between
+#pragma unroll 1
+          for (int k = b + 1; k < quad; ++k) after += block[k];
+          const float u = scan_exp2(after);
           const uint64_t u2 = pair(u, u);
           const float4* v = reinterpret_cast<const float4*>(g + 2 * kScanQ + 32 * b);
           tmem_wait_ld();
@@ -879,7 +885,8 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       fence_proxy_async_smem();
       arrive(kBHFull);
       if (!(ok = wait(kBGateFull + st, c >> 1, kStatusMmaTimeout))) break;
-      const float decay = scan_exp2(totals[st]);
+      const float4 block = blocks[st];
+      const float decay = scan_exp2((block.x + block.y) + (block.z + block.w));
       const uint64_t d2 = pair(decay, decay);
       arrive(kBGateEmpty + st);
       if (!(ok = wait(kBDsFull, c, kStatusMmaTimeout))) break;
@@ -920,7 +927,11 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       const int st = c & 1, n = chunk_len(c);
       uint8_t* stage = smem + st * kScStage;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
-      const float w = scan_exp2(reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[row]);
+      const float* g = reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage);
+      float after = g[kScanQ + row];
+#pragma unroll 1
+      for (int k = quad + 1; k < 4; ++k) after += reinterpret_cast<const float*>(blocks + st)[k];
+      const float w = g[row] * scan_exp2(after);
       arrive(kBGateEmpty + st);
       if (!wait(kBFullX + st, c >> 1, kStatusTmaTimeout)) break;
       if (n < kScanQ) {   // a last, short chunk: what lies past it must not count
@@ -952,8 +963,12 @@ gdn_ssm_scan_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
       const int st = c & 1, n = chunk_len(c);
       uint8_t* stage = smem + st * kScStage;
       if (!wait(kBGateFull + st, c >> 1, kStatusMmaTimeout)) break;
-      const float e = scan_exp2(
-          totals[st] - reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row]);
+      const float* block = reinterpret_cast<const float*>(blocks + st);
+      float since = block[quad] -
+                    reinterpret_cast<const float*>(smem + kScGate + st * kScGateStage)[kScanQ + row];
+#pragma unroll 1
+      for (int k = 0; k < quad; ++k) since += block[k];
+      const float e = scan_exp2(since);
       arrive(kBGateEmpty + st);
       if (!wait(kBFullX + st, c >> 1, kStatusTmaTimeout)) break;
       uint4 x[8];   // kept here so that the stage can be refilled early

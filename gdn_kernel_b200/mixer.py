@@ -135,8 +135,10 @@ def gdn_ssm_prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, output, n
     ``gdn_short_conv``.  workspace: a uint8 CUDA tensor of at least
     ``ssm_prefill_workspace_bytes`` bytes (allocated here when omitted).
 
-    A NaN or infinity in one token's operands can reach outputs of earlier
-    tokens of its chunk, as the products run over whole chunks.
+    A NaN or infinity in a token's x, or a NaN in its dt, can reach outputs of
+    earlier tokens of its sequence in the same chunk of 128, as the products run
+    over whole chunks.  Where decays have left nothing of a token (2^-300), a NaN
+    or infinity of it may reach later tokens and the new state or not.
     """
     ffi = _ffi or _load()
     if workspace is None and x.dim() == 3:

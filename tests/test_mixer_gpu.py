@@ -244,6 +244,43 @@ def test_scan_strong_decay_and_zero_state():
     run_scan([400, 129], 4, 64, 1, 128, strong=True, state=False)
 
 
+# Steep tokens: on top of the roundings, a weight is the exponential of a difference of two
+# sums of up to 32 decays of at most 300 in base 2, off by 2^-10 each.
+STEEP_REL = PROMPT_REL + 2.0 ** -9
+
+
+@pytest.mark.parametrize("size", [10.0, 100.0, 1e4, 1e6, 1e30])
+@pytest.mark.parametrize("where", ["one", "some", "all"])
+@pytest.mark.parametrize("lens", [[200, 70], [1500]])
+def test_scan_steep_tokens(size, where, lens):
+    """Steps that leave nothing of the state, between ordinary ones: what they decay must
+    not cost the weights of the tokens beside them."""
+    x, dt, A_log, B, C, D, bias = scan_inputs(sum(lens), 3, 64, 1, 128, seed=71)
+    at = {"one": slice(100, 101), "some": slice(33, 160, 3), "all": slice(None)}[where]
+    dt[at] = size
+    cu, st = offsets(lens), rand(len(lens), 3, 64, 128, std=0.5, seed=72)
+    out, ns = torch.empty_like(x).contiguous(), torch.empty_like(st)
+    M.gdn_ssm_prefill(x, dt, A_log, B, C, D, bias, st, cu, out, ns)
+    want, wp, mag, pmag = O.scan(x, dt, A_log, B, C, D, bias, st, cu, ns)
+    check(out, want, mag, STEEP_REL, "output")
+    check(ns, wp, pmag, PROMPT_STATE_REL, "state")
+    status_clean()
+
+
+def test_scan_infinite_step_stays_with_its_token_and_those_after():
+    x, dt, A_log, B, C, D, bias = scan_inputs(300, 3, 64, 1, 128, seed=73)
+    cu, at = offsets([300]), 170
+    clean, _ = M.ssm_prefill(x, dt, A_log, B, C, D, bias, None, cu)
+    dt[at, 1] = float("inf")
+    out, _ = M.ssm_prefill(x, dt, A_log, B, C, D, bias, None, cu)
+    assert torch.equal(out[:, [0, 2]], clean[:, [0, 2]]) and torch.equal(out[:128, 1], clean[:128, 1])
+    want, _, mag, _ = O.scan(x[:at], dt[:at], A_log, B[:at], C[:at], D, bias, None, [0, at],
+                             torch.zeros(1, 3, 64, 128))
+    check(out[:at], want, mag, STEEP_REL, "output before")
+    assert not torch.isfinite(out[at, 1]).any()
+    status_clean()
+
+
 def test_scan_pool_slots_and_flags():
     slots = torch.tensor([4, -1, 0, 6], dtype=torch.int64).cuda()
     has = torch.tensor([1, 1, 0, 1], dtype=torch.uint8).cuda()
