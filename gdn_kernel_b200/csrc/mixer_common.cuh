@@ -87,13 +87,12 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-// sigmoid(v) = 1 / (1 + 2^(-v log2 e)) and v sigmoid(v), two at a time: one
-// reciprocal of both denominators' product serves the two, which takes a quarter
-// of the special-function operations off the path that bounds an activation.
-// The exponent stops at 62 so that the product stays finite, and the 2^-62 that
-// sigmoid stops at is taken off, exactly, so that a closed gate is 0 (where sigmoid
-// is small but not yet 0, that is an error of 2^-62).  A NaN reaches only its own
-// result, through silu.
+// sigmoid(v) = 1 / (1 + 2^(-v log2 e)) and v sigmoid(v), two at a time.  The rounded
+// exponent leaves 1.5 |v| 2^-24 of the result, the rest a few units; a NaN stays one,
+// and below -87 sigmoid is 0.  One reciprocal of both denominators' product is no
+// faster (8192 tokens of 8192 channels: 49.1 us against 48.5 with one each; gated norm
+// of 8192 x 4096: 36.5 against 36.7), and needs bounds on the exponents that lose small
+// gates and NaNs, or a branch (50.4 and 39.5 us).
 __device__ __forceinline__ float fast_exp2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -107,18 +106,15 @@ __device__ __forceinline__ float fast_rcp(float v) {
 __device__ __forceinline__ uint64_t sigmoid2(uint64_t v) {
   constexpr float kMinusLog2e = -1.4426950408889634f;
   const float2 t = unpair(mul2(v, pair(kMinusLog2e, kMinusLog2e)));
-  const uint64_t d = add2(pair(fast_exp2(fminf(t.x, 62.0f)), fast_exp2(fminf(t.y, 62.0f))),
-                          pair(1.0f, 1.0f));
-  const float2 f = unpair(d);
-  const float r = fast_rcp(f.x * f.y);
-  constexpr float kFloor = -2.168404344971009e-19f;   // -2^-62
-  return fma2(pair(f.y, f.x), pair(r, r), pair(kFloor, kFloor));
+  const float2 f =
+      unpair(add2(pair(fast_exp2(t.x), fast_exp2(t.y)), pair(1.0f, 1.0f)));
+  return pair(fast_rcp(f.x), fast_rcp(f.y));
 }
 __device__ __forceinline__ uint64_t silu2(uint64_t v) { return mul2(v, sigmoid2(v)); }
 __device__ __forceinline__ float sigmoid_f(float v) {
-  return v != v ? v : fast_rcp(1.0f + fast_exp2(-1.4426950408889634f * v));
+  return fast_rcp(1.0f + fast_exp2(-1.4426950408889634f * v));
 }
-__device__ __forceinline__ float silu_f(float v) { return unpair(silu2(pair(v, 0.0f))).x; }
+__device__ __forceinline__ float silu_f(float v) { return v * sigmoid_f(v); }
 
 // Elements of a 16-byte vector.
 template <typename T> constexpr int kLanes = 16 / static_cast<int>(sizeof(T));

@@ -561,6 +561,48 @@ def test_gated_norm_extremes():
     assert M.gated_norm(x[:0], gate[:0], None).shape == (0, 256)
 
 
+@pytest.mark.parametrize("activation", ["silu", "sigmoid"])
+@pytest.mark.parametrize("norm_first", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width,group", [(256, 64), (1024, 1024), (154, 77)])
+def test_gated_norm_keeps_a_nan_gate(activation, norm_first, dtype, width, group):
+    """Of any alignment: a NaN in a gate is its element's, or through the sum of squares
+    its group's, and no other's."""
+    x, gate = rand(3, width, dtype=dtype), rand(3, width, dtype=dtype, seed=1)
+    want = O.gated_norm(x, gate, None, group, 1e-6, activation, norm_first)
+    gate[1, 5] = float("nan")
+    out = M.gated_norm(x, gate, None, group_size=group, activation=activation,
+                       norm_first=norm_first)
+    hit = torch.zeros(3, width, dtype=torch.bool)
+    hit[1, slice(5, 6) if norm_first else slice(0, group)] = True
+    assert out[hit].isnan().all()
+    check(out[~hit], want[~hit], want[~hit].abs(), NORM_REL, "output")
+
+
+@pytest.mark.parametrize("activation", ["silu", "sigmoid"])
+@pytest.mark.parametrize("width", [256, 77])
+def test_far_ends_of_activations(activation, width):
+    """In fp32, relative to the result, down to gates of -80.  The exponent's rounding
+    leaves 1.5 |v| 2^-24; the norm and the rest 2^-18 as above."""
+    v = torch.linspace(-80, 80, 6 * width).view(6, width)[:, torch.randperm(
+        width, generator=torch.Generator().manual_seed(3))].cuda()
+    x = rand(6, width).abs() + 0.5
+    rel = (2.0 ** -18 + 1.5 * 2.0 ** -24 * v.abs().double()).cpu()
+    for norm_first in (True, False):
+        out = M.gated_norm(x, v, None, activation=activation, norm_first=norm_first).cpu().double()
+        want = O.gated_norm(x, v, None, width, 1e-6, activation, norm_first)
+        normal = want.abs() > 1e-36
+        assert normal.sum() > 0.9 * normal.numel()
+        # before the norm, the largest gates' errors are in the sum too
+        bound = rel if norm_first else rel + rel.max()
+        assert ((out - want).abs() <= bound * want.abs())[normal].all()
+    if activation == "silu":                  # the same of a convolution of one tap
+        w = torch.tensor([0.0, 1.0]).repeat(width, 1).cuda()
+        out, _ = M.short_conv(v, w, None, None, offsets([6]))
+        want, _, _ = O.short_conv(v, w, None, None, [0, 6], torch.zeros(1, 1, width))
+        assert ((out.cpu().double() - want).abs() <= rel * want.abs()).all()
+
+
 @pytest.mark.parametrize("dtype,rdt", [(BF, BF), (BF, F32), (HF, HF), (HF, F32), (F32, F32)])
 @pytest.mark.parametrize("width", [8, 256, 520, 1000, 2048, 5000, 8192, 33, 36864])
 @pytest.mark.parametrize("post", [True, False])
