@@ -37,6 +37,24 @@ bool wide_rows(const void* p, long long stride, int size) {
   return aligned(p, 16) && stride * size % 16 == 0;
 }
 
+// Whether any element of `rows` rows at a is one of those at b.  Rows of the same
+// stride may lie side by side; with other strides it counts if the spans meet.
+bool rows_overlap(const void* a, long long a_stride, const void* b, long long b_stride,
+                  long long rows, long long width, int size) {
+  if (rows == 0) return false;
+  const long long pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+  const long long row = width * size;
+  if (pb >= pa + (rows - 1) * a_stride * size + row || pa >= pb + (rows - 1) * b_stride * size + row)
+    return false;
+  if (rows == 1 || a_stride != b_stride) return true;
+  // b's row i starts `into` bytes after the start of a's row i + by
+  const long long stride = a_stride * size, delta = pb - pa;
+  const long long by = delta >= 0 ? delta / stride : -((stride - 1 - delta) / stride);
+  const long long into = delta - by * stride;
+  return (into < row && by < rows && -by < rows) ||
+         (stride - into < row && by + 1 < rows && -by - 1 < rows);
+}
+
 // ------------------------------------------------------------ short convolution
 template <typename T, int V, int W>
 void launch_conv(const ConvParams& p, unsigned grid, bool step, cudaStream_t st) {
@@ -352,6 +370,9 @@ extern "C" int gdn_b200_short_conv(const void* x, int64_t x_stride, const void* 
     return invalid("null pointer argument");
   if (total_tokens > 1 && (x_stride < channels || output_stride < channels))
     return invalid("rows must not overlap");
+  // blocks read rows that are others' to write
+  if (rows_overlap(x, x_stride, output, output_stride, total_tokens, channels, element_size(dtype)))
+    return invalid("output must not overlap x");
   if (!state_indices && pool_size < num_seqs)
     return invalid("the states hold fewer rows than there are sequences");
   if (!aligned(cu_seqlens, cu_seqlens_is_int64 ? 8 : 4) ||

@@ -78,6 +78,25 @@ def test_nothing_to_do_is_no_error(fn, kw):
     assert lib.gdn_b200_last_error() == b""
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="its addresses hold nothing")
+@pytest.mark.parametrize("rows,width,stride,start", [
+    (9, 64, 64, 0), (9, 64, 64, 5 * 64), (9, 64, 64, -8 * 64), (9, 64, 64, 575), (9, 64, 64, -575),
+    (9, 64, 200, 63), (9, 64, 200, -63), (9, 64, 200, 137), (9, 64, 200, 8 * 200 + 63),
+    (1, 64, 64, 10), (9, 64, 200, 64), (9, 64, 200, 136), (9, 64, 200, -64), (9, 64, 200, -136),
+    (9, 64, 64, 576), (9, 64, 64, -576), (9, 64, 200, 8 * 200 + 64), (9, 64, 200, 9 * 200),
+    (9, 64, 200, 9 * 200 - 63), (1, 64, 64, 64), (9, 64, 200, 3 * 200 + 100)])
+def test_convolution_output_over_its_input(rows, width, stride, start):
+    """Refused exactly where an element of a row is one of another."""
+    a = {r * stride + c for r in range(rows) for c in range(width)}
+    b = {start + e for e in a}
+    lib, x = _lib.load(), 1 << 20
+    one = ctypes.c_void_p(256)
+    rc = lib.gdn_b200_short_conv(ctypes.c_void_p(x), stride, one, Z, Z, one, 0, Z, 0, Z, 1,
+                                 ctypes.c_void_p(x + 2 * start), stride, one, 1, rows, 1, width, 4,
+                                 _lib.BF16, Z)
+    assert (rc == BAD and b"overlap" in lib.gdn_b200_last_error()) == bool(a & b)
+
+
 @pytest.mark.parametrize("seqs,tokens,H,P,N", [
     (1, 512, 8, 1, 64), (1, 512, 8, 32, 64), (1, 512, 8, 63, 128), (1, 512, 8, 96, 64),
     (1, 512, 8, 256, 64), (1, 512, 8, 64, 32), (1, 512, 8, 64, 0), (1, 512, 0, 64, 64),

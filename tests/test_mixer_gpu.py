@@ -148,6 +148,28 @@ def test_short_conv_ignores_values_of_other_sequences():
     assert torch.equal(out[33:], clean[33:]) and torch.isfinite(ns[1]).all()
 
 
+def test_short_conv_output_beside_x_and_not_over_it():
+    T, D = 70, 64
+    buf = rand(T + 3, 2 * D, dtype=BF)
+    x, w, cu = buf[:T, :D], rand(D, 4, dtype=BF), offsets([T])
+    want, new = M.short_conv(x, w, None, None, cu)
+    ns = torch.empty_like(new)
+    keep = buf.clone()
+    for over in (x, buf[:T, 1:D + 1], buf[:T, D - 1:2 * D - 1], buf[3:, :D], buf[2:T + 2, D - 8:2 * D - 8],
+                 buf.view(-1)[:T * D].view(T, D)):
+        with pytest.raises(ValueError, match="overlap"):
+            M.gdn_short_conv(x, w, None, None, cu, over, ns)
+    assert torch.equal(buf, keep)
+    for beside in (buf[:T, D:], buf[3:, D:]):       # the other columns of the same rows, or of others
+        M.gdn_short_conv(x, w, None, None, cu, beside, ns)
+        assert torch.equal(beside, want) and torch.equal(ns, new) and torch.equal(x, keep[:T, :D])
+    one = rand(2, D, dtype=BF)
+    M.gdn_short_conv(one[:1], w, None, None, offsets([1]), one[1:], ns)
+    with pytest.raises(ValueError, match="overlap"):
+        M.gdn_short_conv(one[:1], w, None, None, offsets([1]), one[:1], ns)
+    status_clean()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("batch,channels,width", [(1, 64, 4), (7, 1000, 3), (33, 73, 2),
                                                   (64, 8192, 4)])
