@@ -37,18 +37,23 @@ bool wide_rows(const void* p, long long stride, int size) {
   return aligned(p, 16) && stride * size % 16 == 0;
 }
 
+// Whether rows of `wa` bytes every `sa` bytes from a, and rows of wb every sb from b, span
+// memory that they share.
+bool spans_meet(const void* a, long long sa, long long wa, const void* b, long long sb,
+                long long wb, long long rows) {
+  const long long pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+  return rows > 0 && pb < pa + (rows - 1) * sa + wa && pa < pb + (rows - 1) * sb + wb;
+}
+
 // Whether any element of `rows` rows at a is one of those at b.  Rows of the same
 // stride may lie side by side; with other strides it counts if the spans meet.
 bool rows_overlap(const void* a, long long a_stride, const void* b, long long b_stride,
                   long long rows, long long width, int size) {
-  if (rows == 0) return false;
-  const long long pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
-  const long long row = width * size;
-  if (pb >= pa + (rows - 1) * a_stride * size + row || pa >= pb + (rows - 1) * b_stride * size + row)
-    return false;
+  const long long row = width * size, stride = a_stride * size;
+  if (!spans_meet(a, stride, row, b, b_stride * size, row, rows)) return false;
   if (rows == 1 || a_stride != b_stride) return true;
   // b's row i starts `into` bytes after the start of a's row i + by
-  const long long stride = a_stride * size, delta = pb - pa;
+  const long long delta = reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a);
   const long long by = delta >= 0 ? delta / stride : -((stride - 1 - delta) / stride);
   const long long into = delta - by * stride;
   return (into < row && by < rows && -by < rows) ||
@@ -509,6 +514,12 @@ extern "C" int gdn_b200_ssm_prefill(const void* x, int64_t x_stride, const void*
   if (total_tokens > 0) {
     if (int rc = check_ssm_rows(p)) return rc;
     if (!aligned(output, 32)) return invalid("output needs 32-byte alignment");
+    // pieces of a sequence run side by side, and read tokens that others may have written
+    const long long row = 2LL * num_heads * head_dim, group_row = 2LL * num_groups * state_dim;
+    if (spans_meet(x, 2 * x_stride, row, output, row, row, total_tokens) ||
+        spans_meet(B, 2 * b_stride, group_row, output, row, row, total_tokens) ||
+        spans_meet(C, 2 * c_stride, group_row, output, row, row, total_tokens))
+      return invalid("output must not overlap x, B or C");
   }
   if (int rc = lib_device(&p.status, &sms)) return rc;
   if (total_tokens <= kScanShort * num_seqs)

@@ -130,10 +130,11 @@ def gdn_ssm_prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, output, n
     x: [T, H, P] bf16; dt: [T, H] bf16; B, C: [T, G, N] bf16 (head h reads group
     h // (H // G)), each with a free token stride of 16-byte multiples (dt: any);
     A_log: [H] fp32; D, dt_bias: [H] fp32 or None; P and N are 64 or 128;
-    state: [S, H, P, N] fp32 or None (zero); output: [T, H, P] bf16; new_state:
-    [S, H, P, N] fp32 (may be state); cu_seqlens, state_indices, has_state as in
-    ``gdn_short_conv``.  workspace: a uint8 CUDA tensor of at least
-    ``ssm_prefill_workspace_bytes`` bytes (allocated here when omitted).
+    state: [S, H, P, N] fp32 or None (zero); output: [T, H, P] bf16 (not
+    overlapping the inputs); new_state: [S, H, P, N] fp32 (may be state);
+    cu_seqlens, state_indices, has_state as in ``gdn_short_conv``.  workspace: a
+    uint8 CUDA tensor of at least ``ssm_prefill_workspace_bytes`` bytes
+    (allocated here when omitted).
 
     A NaN or infinity in a token's x, or a NaN in its dt, can reach outputs of
     earlier tokens of its sequence in the same chunk of 128, as the products run

@@ -302,7 +302,8 @@ int gdn_b200_short_conv_step(const void* x, int64_t x_stride, const void* weight
  *   A_log [H] fp32;  D, dt_bias [H] fp32 or NULL (zero)
  *   state, new_state [pool_size, H, P, N] fp32; state NULL = zero; may be the same
  *   head_dim P in {64, 128}, state_dim N in {64, 128}, H % G == 0
- * x, B and C need 16-byte aligned rows, output a 32-byte aligned start.  An empty sequence keeps its state.
+ * x, B and C need 16-byte aligned rows, output a 32-byte aligned start and memory of
+ * its own.  An empty sequence keeps its state.
  * The workspace (gdn_b200_ssm_prefill_workspace_size() bytes, 256-byte aligned)
  * lets long sequences run in pieces side by side; NULL is allowed.  Calls that
  * may overlap need workspaces of their own.

@@ -445,6 +445,27 @@ def test_scan_of_nothing():
     status_clean()
 
 
+@pytest.mark.parametrize("T", [8, 300, 3000])
+def test_scan_output_over_x_is_refused(T):
+    """Of any length: pieces of the longest would read what others have written."""
+    ins = scan_inputs(T, 2, 64, 1, 128)
+    x = ins[0].contiguous()
+    ns, keep = torch.zeros(1, 2, 64, 128).cuda(), x.clone()
+    with pytest.raises(ValueError, match="overlap"):
+        M.gdn_ssm_prefill(x, *ins[1:], None, offsets([T]), x, ns)
+    assert torch.equal(x, keep) and (ns == 0).all()
+    bc = torch.zeros(T, 2, 128, dtype=BF).cuda()
+    for k in (3, 4):
+        part = list(ins)
+        part[k] = bc[:, :1]
+        with pytest.raises(ValueError, match="overlap"):
+            M.gdn_ssm_prefill(*part, None, offsets([T]), bc.view(-1)[:T * 128].view(T, 2, 64), ns)
+    both = torch.cat([x, torch.zeros_like(x)])
+    M.gdn_ssm_prefill(both[:T], *ins[1:], None, offsets([T]), both[T:], ns)
+    want, _ = M.ssm_prefill(*ins, None, offsets([T]))
+    assert torch.equal(both[T:], want)
+
+
 def test_scan_bad_offsets_and_slots():
     ins = scan_inputs(40, 4, 64, 1, 64)
     out = torch.zeros(40, 4, 64, dtype=BF).cuda()
