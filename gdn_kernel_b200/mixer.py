@@ -142,7 +142,7 @@ def gdn_ssm_prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, output, n
     or infinity of it may reach later tokens and the new state or not.
     """
     ffi = _ffi or _load()
-    if workspace is None and x.dim() == 3:
+    if workspace is None and x.dim() == 3 and B.dim() == 3:
         T, H, P = x.shape
         need = ffi.ssm_prefill_workspace(cu_seqlens.numel() - 1, T, H, P, B.shape[-1])
         if need:

@@ -208,6 +208,14 @@ def test_python_refuses(call, kw, words):
         call(**kw)
 
 
+@pytest.mark.parametrize("kw,words", [
+    (dict(B=z()), "B: must be"), (dict(B=z(128)), "B: must be"), (dict(x=z()), "x: must be"),
+    (dict(cu=torch.tensor(4)), "cu_seqlens"), (dict(cu=z(0, dtype=I32)), "cu_seqlens")])
+def test_scan_refuses_what_has_no_sizes_to_plan_for(kw, words):
+    with pytest.raises(ValueError, match=words):
+        scan(**kw)
+
+
 @pytest.mark.parametrize("P", [1, 32, 63])
 def test_python_refuses_small_heads_before_planning(P):
     with pytest.raises(ValueError, match="head_dim"):
