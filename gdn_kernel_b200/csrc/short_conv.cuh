@@ -163,7 +163,7 @@ __device__ __forceinline__ void short_sequence(const ConvParams& p, int seq, int
 // (8192 tokens of 8192 channels: 63 us).  V = 1: plain loads.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const ConvParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t conv_smem[];
   constexpr bool kStaged = V == kConvVec;
   constexpr int kRow = kConvThreads * V;          // elements of a staged row
   const int c0 = static_cast<int>(blockIdx.x % p.chan_blocks) * kRow;
@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
   const int t1 = min(t0 + p.tile, tokens);
   const int r0 = max(t0 - (W - 1), 0);            // rows staged: [r0, r1)
   const int r1 = min(t1 + W - 2, tokens);
-  const T* rows = reinterpret_cast<const T*>(smem + 128) + threadIdx.x * V;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem);
+  const T* rows = reinterpret_cast<const T*>(conv_smem + 128) + threadIdx.x * V;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(conv_smem);
   // The sequences of the tile that are done here, 32 looked at together, a lane
   // each: work(sequence, its bounds) by whole warps.
   const int lane = threadIdx.x & 31;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kConvThreads) gdn_short_conv_kernel(const Conv
       for (int i = threadIdx.x; i < n; i += 32)
         asm volatile(
             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-            ::"r"(smem_u32(smem + 128 + static_cast<size_t>(i) * kRow * sizeof(T))),
+            ::"r"(smem_u32(conv_smem + 128 + static_cast<size_t>(i) * kRow * sizeof(T))),
             "l"(static_cast<const T*>(p.x) + static_cast<long long>(r0 + i) * p.x_stride + c0), "r"(bytes),
             "r"(smem_u32(bar))
             : "memory");
