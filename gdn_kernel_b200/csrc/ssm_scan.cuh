@@ -212,13 +212,14 @@ __device__ inline void scan_item(const ScanParams& sp, int item, ScanItem* out) 
   *out = it;
 }
 
-// Waits are warp-uniform and bounded: so many tries, each of which sleeps up to 4 us
-// (without a hint; one of a microsecond made the whole 2-3 % slower), so half a second
-// at most and milliseconds at the least.  None spans more than a few chunks' work.
-// The first to run out raises the abort flag, which ends every role's loop.  (A count
-// takes a fraction of the code of a clock, and the roles' loops have to fit the
-// instruction cache together.)
-constexpr int kScanWaitTries = 1 << 17;
+// Waits are warp-uniform and bounded: so many tries, each of which sleeps 4 us here
+// (256 of them took 1.02 ms for one warp and for 28; with a hint of a microsecond the
+// whole was 2-3 % slower), so 2.1 seconds, near the limit of the GDN kernels' waits.
+// A system that let tries return at once would leave 10 ms, a thousand times what
+// the longest wait, a few chunks' work, takes.  The first to run out raises the
+// abort flag, which ends every role's loop.  (A count takes a fraction of the code of
+// a clock, and the roles' loops have to fit the instruction cache together.)
+constexpr int kScanWaitTries = 1 << 19;
 __device__ __forceinline__ bool scan_try_wait(uint32_t addr, uint32_t parity) {
   uint32_t ok;
   asm volatile(
