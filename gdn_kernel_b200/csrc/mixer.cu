@@ -216,10 +216,12 @@ int ssm_recurrent_call(const SsmParams& p, int32_t state_dim, int64_t entries, c
   return launched("selective scan launch");
 }
 
-// Prompts of up to so many tokens on average run token by token: a chunk costs the
-// same however few tokens it has.  64 heads of 64, state 128, token by token / in
-// chunks: 1 x 8 tokens 7.2 / 8.5 us, 1 x 16 11.5 / 8.4, 8 x 8 16 / 31, 8 x 24
-// 38 / 31, 64 x 4 77 / 204, 64 x 16 180 / 205, 64 x 24 240 / 205.
+// Prompts of up to so many tokens on average (and calls without tokens) run token by
+// token: a chunk costs the same however few tokens it has.  The average decides for
+// the whole call, as lengths are on the device: one long prompt beside many short
+// ones may run token by token too.  Sequences of equal lengths, 64 heads of 64, state
+// 128, token by token / in chunks: 1 x 8 tokens 7.2 / 8.5 us, 1 x 16 11.5 / 8.4,
+// 8 x 8 16 / 31, 8 x 24 38 / 31, 64 x 4 77 / 204, 64 x 16 180 / 205, 64 x 24 240 / 205.
 constexpr int kScanShort = 10;
 
 // The scan kernels' shared memory is above the default limit: raised once per
@@ -305,22 +307,10 @@ int ssm_scan_call(const SsmParams& p, int32_t state_dim, int64_t seqs, void* wor
   ScanPlan plan = scan_plan(seqs, p.tokens, p.heads, p.head_dim, state_dim);
   if (!workspace || workspace_bytes < plan.bytes || plan.max_full * plan.parts + seqs > 65535)
     plan = ScanPlan{0, 1, 0, 0, 0};
-  // Without tokens every sequence is empty and nothing is loaded; the maps still
-  // need an extent, so they describe one token's worth of new_state.
-  const bool some = p.tokens > 0;
   CUtensorMap tx, tb, tc;
-  if (int rc = lib_token_map(&tx, some ? static_cast<const void*>(p.x) : p.new_state, p.head_dim,
-                             some ? p.heads : 1, some ? p.tokens : 1,
-                             some ? p.x_stride : p.head_dim, kScanQ))
-    return rc;
-  if (int rc = lib_token_map(&tb, some ? static_cast<const void*>(p.B) : p.new_state, state_dim,
-                             some ? p.groups : 1, some ? p.tokens : 1,
-                             some ? p.b_stride : state_dim, kScanQ))
-    return rc;
-  if (int rc = lib_token_map(&tc, some ? static_cast<const void*>(p.C) : p.new_state, state_dim,
-                             some ? p.groups : 1, some ? p.tokens : 1,
-                             some ? p.c_stride : state_dim, kScanQ))
-    return rc;
+  if (int rc = lib_token_map(&tx, p.x, p.head_dim, p.heads, p.tokens, p.x_stride, kScanQ)) return rc;
+  if (int rc = lib_token_map(&tb, p.B, state_dim, p.groups, p.tokens, p.b_stride, kScanQ)) return rc;
+  if (int rc = lib_token_map(&tc, p.C, state_dim, p.groups, p.tokens, p.c_stride, kScanQ)) return rc;
   ScanParams sp{};
   sp.s = p;
   sp.seg_chunks = plan.seg_chunks;
