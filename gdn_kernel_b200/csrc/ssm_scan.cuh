@@ -251,14 +251,19 @@ struct ScanSync {
   }
 };
 
-// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|), in a few units of 2^-24:
-// the exponent's product is carried in two parts, and with z = e / (2 + e),
-// log1p(e) = 2 atanh(z) = 2 (z + z^3 / 3 + z^5 / 5 + ...), z <= 1/3, where the
-// terms from z^15 on are below 2^-26 of the sum.
+// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|), in a few units of 2^-24.  The
+// product -|v| log2 e is carried in two parts, head and rest, with log2 e split into
+// its fp32 value and the difference: e = 2^head (1 + rest ln 2), as rest is small.
+// log1p(e) is the series of its hyperbolic arctangent, with z = e / (2 + e):
+// 2 atanh(z) = 2 (z + z^3 / 3 + z^5 / 5 + ...), z <= 1/3, where the terms from z^15
+// on are below 2^-26 of the sum.
 __device__ __forceinline__ float scan_step_size(float v) {
+  constexpr double kLog2e = 1.4426950408889634;
+  constexpr float kHead = static_cast<float>(kLog2e);
+  constexpr float kRest = static_cast<float>(kLog2e - static_cast<double>(kHead));
   const float a = fmaxf(-fabsf(v), -150.0f);   // e underflows below; and -inf is a value
-  const float hi = a * 1.4426950408889634f;
-  const float lo = fmaf(a, 1.4426950408889634f, -hi) + a * 1.925963033500e-8f;
+  const float hi = a * kHead;
+  const float lo = fmaf(a, kHead, -hi) + a * kRest;
   float e = scan_exp2(hi);
   e = fmaf(e, lo * 0.6931471805599453f, e);
   const float z = __fdividef(e, 2.0f + e);
