@@ -3,12 +3,15 @@ scan layers in turn, prompts first, then one token per sequence at a time.
 
 Every layer is  residual add + norm -> projection -> short convolution -> recurrence
 -> gated norm -> projection.  The projections are plain matrix products with random
-weights; everything between them is one call of this package each:
+weights; the operators between them are calls of this package:
 
     add_norm, short_conv / short_conv_step, prefill / gdn_decode_pool (GDN layers) or
     ssm_prefill / ssm_step (scan layers), gated_norm
 
-The states stay in pools with a slot per sequence, updated in place.
+A GDN layer norms q and k with two more gated_norm calls, copies v, a and b (its calls
+take contiguous tensors), and stores a prompt's states to their slots itself; a scan
+layer reads column slices and slots as they are.  The states stay in pools with a slot
+per sequence, updated in place by the steps.
 
     python examples/hybrid_stack.py            # prompts, then steps; checks the two agree
 """

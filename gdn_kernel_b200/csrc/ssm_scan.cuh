@@ -40,8 +40,8 @@
 // Rows past a sequence's end hold other tokens: X, B and w X rows are zeroed
 // there, so nothing of them (not even a NaN) enters a product's sum.
 //
-// Measured: 8192 tokens, 64 heads of 64, state 128, 98 us with the kernel of the
-// pieces' states (20 us); 20011 ragged tokens of 32 heads of 128, state 64, 161 us.
+// Measured: 8192 tokens, 64 heads of 64, state 128, 96 us with the kernel of the
+// pieces' states (20 us); 20011 ragged tokens of 32 heads of 128, state 64, 163-170.
 // A chunk takes about 4000 clocks, its shared-memory traffic 3070 (384 KB: 208 of
 // product operands, 80 of arriving tiles, 96 of x, w X and h), the tensor pipe is
 // active for 2750; the rest is handing over.  128 tokens a chunk, because products
